@@ -24,6 +24,8 @@ GEMM_HALF_SMS = 256
 GEMM_AUX_ROUNDED = 512
 GEMM_AUX_FAST = 1024
 FLASH_OPERANDS_ROUNDED = 1
+TYPE_FP32, TYPE_BF16, TYPE_FP16 = 0, 1, 2
+E_ARG = 1
 E_UNSUPPORTED = 3
 E_TIMEOUT = 4
 E_LIMIT = 6
@@ -43,6 +45,37 @@ class DdpTiming(C.Structure):
 
 class KernelEntry(C.Structure):
     _fields_ = [("id", _i), ("name", C.c_char_p), ("fn", _p), ("note", C.c_char_p), ("tol", _d)]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("k", _p), ("v", _p), ("page_stride", _ll), ("token_stride", _ll), ("head_stride", _ll)] + \
+               [(n, _i) for n in ("type", "pages", "page_size", "heads", "head_size")]
+
+    @classmethod
+    def of(cls, k, v):
+        """The cache in two tensors of the same shape (pages, page size, heads, head size), type and strides (a
+        permuted view where heads lie outside a page's tokens).  It keeps them alive."""
+        types = {"torch.float32": TYPE_FP32, "torch.bfloat16": TYPE_BF16, "torch.float16": TYPE_FP16}
+        if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.dim() != 4 or k.stride(3) != 1 or str(k.dtype) not in types:
+            raise ValueError("k and v: fp32, bf16 or fp16, (pages, page size, heads, head size), alike, elements of a head side by side")
+        c = cls(ptr(k), ptr(v), k.stride(0), k.stride(1), k.stride(2), types[str(k.dtype)], *k.shape)
+        c.tensors = (k, v)
+        return c
+
+
+class LogitRules(C.Structure):
+    _fields_ = [(n, _p) for n in ("history", "history_lens", "prompt_lens", "repetition", "frequency", "presence", "bias_ids", "bias",
+                                  "bias_lens", "allowed")] + [(n, _i) for n in ("history_stride", "bias_stride", "allowed_stride")]
+
+    @classmethod
+    def of(cls, **parts):
+        """The rules in tensors (each optional; history, bias_ids and allowed with a row for each text).  It keeps them alive."""
+        r = cls(**{k: ptr(t) for k, t in parts.items()})
+        for name, stride in (("history", "history_stride"), ("bias_ids", "bias_stride"), ("allowed", "allowed_stride")):
+            if parts.get(name) is not None:
+                setattr(r, stride, parts[name].stride(0))
+        r.tensors = parts
+        return r
 
 
 # name -> (restype, argtypes); must list every function include/bmb.h declares.
@@ -108,6 +141,12 @@ SIGNATURES = {
     "bmb_grad_sumsq_device": (_i, [_p, _z, _p]),
     "bmb_reduce_mean_device": (_i, [_p, _i, _p]),
     "bmb_adamw_update_clipped": (_i, [_p, _p, _p, _p, _z, _f, _f, _f, _f, _f, _i, _p, _f, _f, _p]),
+    "bmb_pages_assign": (_i, [_p] * 11 + [_i] * 5 + [_p]),
+    "bmb_pages_release": (_i, [_p] * 7 + [_i] * 4 + [_p]),
+    "bmb_paged_kv_write": (_i, [C.POINTER(KvCache), _p, _p, _ll, _p, _i, _p]),
+    "bmb_paged_attention_workspace": (_z, [_i] * 3),
+    "bmb_paged_attention": (_i, [_p, _p, _p, C.POINTER(KvCache), _p, _p, _i, _i, _ll, _ll, _i, _f, _p, _z, _p]),
+    "bmb_logits_adjust": (_i, [_p, _p, _i, _i, _ll, C.POINTER(LogitRules), _p]),
     "bmb_ddp_create": (_i, [C.POINTER(_p), _i, C.POINTER(_i)]),
     "bmb_ddp_destroy": (_i, [_p]),
     "bmb_ddp_allreduce": (_i, [_p, C.POINTER(_p), _z]),
@@ -190,6 +229,11 @@ def call(name, *args):
     """Call a status-returning entry point with tensors turned into pointers."""
     conv = [ptr(a) if (a is None or hasattr(a, "data_ptr") or hasattr(a, "ctypes")) else a for a in args]
     check(getattr(lib(), name)(*conv), name)
+
+
+def paged_attention_workspace(heads, kv_heads, head_size):
+    """Bytes of workspace that a call of bmb_paged_attention needs on the current device."""
+    return lib().bmb_paged_attention_workspace(heads, kv_heads, head_size)
 
 
 class Trainer:

@@ -276,6 +276,95 @@ int bmb_adamw_update_clipped(float *params, const float *grads, float *m,
                              int step, const double *d_sumsq, float clip,
                              float div, float *shadow);
 
+/* ---- serving several requests: a paged cache, attention over it, logits before a draw ------------ */
+/* No counterparts in the reference, whose generate() (src/train_gpt.cu:46-102) serves one text.  A step of a program that
+ * answers several requests at once is: bmb_pages_assign (pages and slots for the step's new tokens), per layer
+ * bmb_paged_kv_write and bmb_paged_attention, bmb_logits_adjust before the draw, and bmb_pages_release for requests that end.
+ * None of them allocates, blocks or keeps anything between calls, so all can be captured; sums and softmax statistics are fp32.
+ *
+ * A cache is a pool of pages of page_size tokens each.  Token t of page p has its keys of head h at
+ * k + p * page_stride + t * token_stride + h * head_stride (strides in elements; head_size elements in a row), its values at
+ * the same place of v: [pages][page_size][heads][head_size] and [pages][heads][page_size][head_size] alike, k and v apart or
+ * interleaved.  Both pointers and all strides are multiples of 16 bytes, every stride at least head_size; head_size is
+ * 32, 64 or 128 (BMB_E_UNSUPPORTED otherwise); pages * page_size fits an int (BMB_E_LIMIT).  The slot of that token is
+ * p * page_size + t.  The struct is read during the call only. */
+#define BMB_TYPE_FP32 0
+#define BMB_TYPE_BF16 1
+#define BMB_TYPE_FP16 2
+typedef struct bmb_kv_cache {
+    void *k, *v;
+    long long page_stride, token_stride, head_stride;
+    int type; /* BMB_TYPE_* of the elements */
+    int pages, page_size, heads, head_size;
+} bmb_kv_cache;
+
+/* Pages for the new tokens of n requests, and the slot of each.  Request i has lens[i] tokens in the cache, in the pages of
+ * row i of tables ([n][max_pages]), and gets new_lens[i] more (negative: 0; 1 in a step of decoding, many for a prompt, 0 for
+ * a request that rests).  Pages are popped from the stack free_pages[0 .. *free_count) (clamped to `pages`, the size of the
+ * pool and of that array), from its end, in the order of the requests.  A request that the pool cannot serve, that
+ * would need more than max_pages or whose tokens end beyond max_tokens gets nothing (lens_out tells); after the first
+ * request that the pool cannot serve only those that need no page are served.
+ *   tables     the entries of new pages are written, others are left alone
+ *   lens_out   [n] lens + new_lens, or lens where the request was not served (may be lens itself)
+ *   slots      [max_tokens] of the new tokens, request after request; -1 for tokens of requests not served, for tokens whose
+ *              page is not one of the pool, and behind the last token (where positions is 0 and owners -1)
+ *   positions  [max_tokens] a token's index in its request, owners [max_tokens] the request (each may be NULL)
+ *   starts     [n + 1] where each request's tokens begin and the last one's end, at most max_tokens (may be NULL)
+ *   free_left  pages left on the stack (may be free_count itself); free_pages is not written
+ * All pointers are device pointers, lens and new_lens included; sums of lengths are 64-bit. */
+int bmb_pages_assign(int *tables, int *lens_out, int *slots, int *positions, int *owners, int *starts, int *free_left,
+                     const int *lens, const int *new_lens, const int *free_pages, const int *free_count, int n, int max_pages,
+                     int page_size, int pages, int max_tokens, void *stream);
+/* The pages of the requests with done[i] != 0 go back on the stack, request after request and in the order of their tables:
+ * written from free_pages[*free_count] on, *free_out = the new count (may be free_count itself), lens_out[i] = 0 for
+ * those and lens[i] (at least 0) for the others (may be lens itself).  Entries that are not pages of the pool are left out, and what the stack
+ * (`pages` entries) has no room for.  tables is not written; a page must not be in two tables. */
+int bmb_pages_release(int *free_pages, int *free_out, int *lens_out, const int *free_count, const int *lens, const int *tables,
+                      const int *done, int n, int max_pages, int page_size, int pages, void *stream);
+/* Rows of keys and values (heads * head_size floats each, row_stride floats from one token to the next: 3C for rows of a qkv
+ * product) into the slots of their tokens, rounded to the cache's type (to nearest even; beyond fp16's range: infinity).
+ * Rows whose slot is negative or beyond the pool are left out.  Slots are distinct (of two rows with one slot either may be
+ * found there, or elements of both). */
+int bmb_paged_kv_write(const bmb_kv_cache *cache, const float *k, const float *v, long long row_stride, const int *slots,
+                       int tokens, void *stream);
+/* Attention of one new token of each of n requests over the tokens that the cache holds of it (its own included, once written):
+ * out[i][h] = sum_j softmax_j(scale q[i][h] . k_j) v_j over j < lens[i] (clamped to the table), where heads is a multiple of the
+ * cache's and query head h reads cache head h / (heads / cache->heads).  Rows of q and out are q_stride and out_stride floats
+ * apart (q may lie in rows of a qkv product; out must not overlap it).  lse ([n][heads], may be NULL) receives the natural
+ * logarithm of the sum of exponentials.  Row i of tables ([n][max_pages]) names request i's pages; tokens in pages that are
+ * not of the pool count as absent, and are not read.  Where nothing is left, out is 0 and lse -infinity.
+ * workspace: bmb_paged_attention_workspace bytes on the device, 16-byte aligned, of this call's own until it has run (two
+ * streams, or two graphs that may run at once, have one each); its contents need no preparation and mean nothing afterwards.
+ * Products and sums are of fp32 accuracy whatever the cache's type.  An infinity or NaN in q, or in a key or value that counts,
+ * makes the outputs that it enters NaN. */
+size_t bmb_paged_attention_workspace(int heads, int kv_heads, int head_size);
+int bmb_paged_attention(float *out, float *lse, const float *q, const bmb_kv_cache *cache, const int *tables, const int *lens,
+                        int n, int heads, long long q_stride, long long out_stride, int max_pages, float scale, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
+/* Rules for rows of logits, each part optional (NULL), every array on the device:
+ *   history   [n][history_stride] tokens of each text, the first history_lens[i] count, of those the first prompt_lens[i]
+ *             (NULL: none) are the prompt; entries outside the vocabulary are passed over
+ *   repetition, frequency, presence   [n], need history
+ *   bias_ids, bias   [n][bias_stride], the first bias_lens[i] count; of entries for one token the last; ids outside the vocabulary are passed over
+ *   allowed   [n][allowed_stride] words: bit v % 32 of word v / 32 is 1 where token v may be drawn
+ * Lengths are clamped to their strides. */
+typedef struct bmb_logit_rules {
+    const int *history, *history_lens, *prompt_lens;
+    const float *repetition, *frequency, *presence;
+    const int *bias_ids;
+    const float *bias;
+    const int *bias_lens;
+    const unsigned *allowed;
+    int history_stride, bias_stride, allowed_stride;
+} bmb_logit_rules;
+/* out[i][v] for v < V, rows of both `stride` floats apart (out may be logits itself), in this order:
+ *   x = logits;  v in the text: x > 0 ? x / repetition : x * repetition;  x -= frequency * (times v was drawn);
+ *   v drawn at all: x -= presence;  x += bias;  not allowed: -infinity
+ * every step rounded to fp32 by itself.  Columns from V on are left as they are in out.  A row whose mask allows nothing is -infinity
+ * throughout. */
+int bmb_logits_adjust(float *out, const float *logits, int n, int V, long long stride, const bmb_logit_rules *rules, void *stream);
+
 /* ---- data-parallel all-reduce (src/ddp.h:32-69) ------------------------ */
 typedef struct bmb_ddp_timing {
     double reduce_scatter_ms;
