@@ -145,6 +145,7 @@ SIGNATURES = {
     "bmb_pages_release": (_i, [_p] * 7 + [_i] * 4 + [_p]),
     "bmb_paged_kv_write": (_i, [C.POINTER(KvCache), _p, _p, _ll, _p, _i, _p]),
     "bmb_paged_attention_workspace": (_z, [_i] * 3),
+    "bmb_paged_attention_schedule_check": (_i, [_p] + [_i] * 7 + [C.POINTER(_ll), C.POINTER(_i)]),
     "bmb_paged_attention": (_i, [_p, _p, _p, C.POINTER(KvCache), _p, _p, _i, _i, _ll, _ll, _i, _f, _p, _z, _p]),
     "bmb_logits_adjust": (_i, [_p, _p, _i, _i, _ll, C.POINTER(LogitRules), _p]),
     "bmb_ddp_create": (_i, [C.POINTER(_p), _i, C.POINTER(_i)]),

@@ -1,16 +1,15 @@
 // A paged cache of keys and values, and attention of one new token of each request over its pages.
-#include "common.cuh"
+#include "flash_mma.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <climits>
 #include <cmath>
+#include <type_traits>
+#include <vector>
 
 namespace bmb {
 namespace {
 
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 template <typename T> __device__ __forceinline__ T from_float(float x);
 template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
@@ -29,41 +28,585 @@ __global__ void __launch_bounds__(256) kv_write_k(bmb_kv_cache c, const float *k
     }
 }
 
-// A block for each request and query head; its warps take tokens in turn, a lane HS / 32 elements of each.
+// ---- attention of one token of each request ---------------------------------------------------------------------------
+//
+// out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q . k_j, with running m, sums and outputs in one pass over keys and
+// values, which is all the work there is: 2 to 4 operations a byte for each query head that shares them.  So what counts is that the
+// loads never pause, on every SM alike, whatever the lengths are.
+//
+// Work: the tiles of all requests and cache heads stand in one line, a tile being 4 KB of keys and 4 KB of values, and are cut
+// into equal runs, one for each warp of the GPU.  A warp is on its own: its tiles come by cp.async through a ring of its own, over the
+// borders of heads and requests, and no block-wide barrier stands in the loop.  Heads that lie in several runs are joined, first
+// among the warps of a block, and what reaches over blocks by attend_join_k.  Nothing depends on arrival, so equal calls give equal bits.
+//
+// Arithmetic: warp-level matrix instructions, 8 query heads of one cache head a time, at fp32 accuracy.  Queries and weights are
+// fp32, so each goes in as pieces of the cache's type, whose products with its elements are exact: the 16 rows of an
+// instruction are the 8 rows' first pieces and their second ones, so a row's two sums lie in one lane and are added there.  fp16:
+// two pieces of 11 bits, scaled by a power of two for each row of q (weights by 2^14), kept down to 2^-38 of the row's
+// largest.  bf16: three of 8 bits, the third in an instruction of its own.  fp32: two TF32 pieces (fm, flash_mma.cuh) of queries and
+// weights, and of keys and values as they are read.  Sums over tiles are kept in fp32 registers.  Masked and absent tokens are zeros in
+// shared memory with a weight of zero, whatever the memory there holds.
+constexpr int PA_WARPS = 8, PA_THREADS = 32 * PA_WARPS, PA_STAGES = 3, PA_TILE = 4096, PA_ROWS = 8, PA_MIN_TILES = 1;
+constexpr int PA_STRETCHES = 128;       // stretches of requests whose tiles a block counts, to find where a run begins
+
+// All tiles in a line: requests in order, of each its (virtual) heads, of each its tiles.
+struct Line {
+    long long tiles;
+    int warps;             // runs: warp w has tiles [begin(w), begin(w + 1))
+    __host__ __device__ Line(long long tiles_, int most) : tiles(tiles_), warps((int)(tiles_ / PA_MIN_TILES < most ? tiles_ / PA_MIN_TILES : most)) {
+        if (warps < 1) warps = 1;
+    }
+    __host__ __device__ long long begin(int w) const { return tiles * w / warps; }
+    __host__ __device__ int warp_of(long long tile) const { return (int)(((tile + 1) * warps - 1) / tiles); }
+};
+struct Shape {
+    int n, heads, group, parts, vheads, cap, keys;   // query heads a cache head, its groups of 8, virtual heads in all, longest length, keys a tile
+    __host__ __device__ int length(int len) const { return len < 0 ? 0 : len < cap ? len : cap; }
+    __host__ __device__ int stretch() const { return (n - 1) / PA_STRETCHES + 1; }
+    __host__ __device__ int tiles(int len) const { return (int)(((long long)length(len) + keys - 1) / keys); }
+    // the place in the line of a head's last tile; `before`: tiles (of one head each) of the requests before request `first`
+    __host__ __device__ long long last_tile(const int *lens, int request, int vhead, int first, long long before) const {
+        for (int i = first; i < request; ++i) before += tiles(lens[i]);
+        return before * vheads + (long long)(vhead + 1) * tiles(lens[request]) - 1;
+    }
+};
+// A place in the line.
+struct Place {
+    int request, vhead, tile, tiles, len;
+    // to the tile `in` tiles behind the first one of request r
+    __host__ __device__ void set(const Shape &s, const int *lens, int r, long long in) {
+        for (; r + 1 < s.n && in >= (long long)s.tiles(lens[r]) * s.vheads; ++r) in -= (long long)s.tiles(lens[r]) * s.vheads;
+        request = r;
+        len = s.length(lens[r]);
+        tiles = s.tiles(len);
+        vhead = (int)(in / tiles);
+        tile = (int)(in % tiles);
+    }
+    __host__ __device__ void next(const Shape &s, const int *lens) {
+        if (++tile < tiles) return;
+        tile = 0;
+        if (++vhead < s.vheads) return;
+        vhead = 0;
+        for (tiles = 0; tiles == 0 && ++request < s.n;) {
+            len = s.length(lens[request]);
+            tiles = s.tiles(len);
+        }
+    }
+};
+
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __half) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&c)[4], const float (&a)[4], float b0, float b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])), "r"(__float_as_uint(a[3])),
+                   "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    if (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi, __half) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&v)); }
+__device__ __forceinline__ float2 unpack(uint32_t v, __half) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
+// A pair of fp32 values as pairs of pieces, the nearest value of the type each; `pieces` of them.
+template <typename T, int pieces>
+__device__ __forceinline__ void split(float x, float y, uint32_t (&out)[pieces]) {
+#pragma unroll
+    for (int i = 0; i < pieces; ++i) {
+        out[i] = pack(x, y, T());
+        const float2 v = unpack(out[i], T());
+        x -= v.x;
+        y -= v.y;
+    }
+}
+
+// Rows of a head in the workspace: of a block, the part of the head that it ends (0) and of the one that it begins (1).
+struct Parts {
+    float *o, *m, *l;      // [blocks][2][PA_ROWS][HS], [blocks][2][PA_ROWS]
+    int4 *begun;           // [blocks]: request, virtual head, last block, 1; or w = 0 where the block begins no head that others go on with
+};
+constexpr size_t part_floats(int blocks, int hs) { return (size_t)blocks * 2 * PA_ROWS * (hs + 2); }
+size_t attend_workspace(int blocks, int hs) { return (part_floats(blocks, hs) * sizeof(float) + 15) / 16 * 16 + (size_t)blocks * sizeof(int4); }
+
+struct Attend {
+    float *out, *lse;
+    const float *q;
+    bmb_kv_cache c;
+    const int *tables, *lens;
+    long long q_stride, out_stride;
+    int max_pages;
+    float scale;
+    Shape s;
+    Parts w;
+};
+
 template <typename T, int HS>
-__global__ void __launch_bounds__(256) attend_k(float *out, float *lse, const float *q, bmb_kv_cache c, const int *tables, const int *lens, int heads,
-                                                long long q_stride, long long out_stride, int max_pages, float scale) {
-    constexpr int E = HS / 32, WARPS = 8;
-    __shared__ float m_of[WARPS], l_of[WARPS], o_of[WARPS][HS];
-    const int i = blockIdx.x / heads, h = blockIdx.x % heads, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int len = (int)min((long long)max(lens[i], 0), (long long)max_pages * c.page_size);
-    const T *K = (const T *)c.k + (h / (heads / c.heads)) * c.head_stride, *V = (const T *)c.v + (h / (heads / c.heads)) * c.head_stride;
-    float qr[E], o[E], m = -INFINITY, l = 0.0f;
-    for (int e = 0; e < E; ++e) { qr[e] = q[i * q_stride + h * HS + lane * E + e]; o[e] = 0.0f; }
-    for (int t = w; t < len; t += WARPS) {
-        const int page = tables[(size_t)i * max_pages + t / c.page_size];
-        if (page < 0 || page >= c.pages) continue;
-        const long long at = page * c.page_stride + (t % c.page_size) * c.token_stride + lane * E;
-        float s = 0.0f;
-        for (int e = 0; e < E; ++e) s = fmaf(qr[e], to_float(K[at + e]), s);
-        s = warp_sum(s) * scale;
-        const float mn = fmaxf(m, s), keep = expf(m - mn), p = expf(s - mn);
-        l = l * keep + p;
-        for (int e = 0; e < E; ++e) o[e] = fmaf(p, to_float(V[at + e]), o[e] * keep);
-        m = mn;
+__global__ void __launch_bounds__(PA_THREADS, 1) attend_k(const __grid_constant__ Attend p) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+    constexpr int KEYS = PA_TILE / (HS * (int)sizeof(T)), NT = KEYS / 8;         // keys a tile, and tiles of 8
+    constexpr int UNITS = HS * (int)sizeof(T) / 16;                              // 16-byte units of a row
+    constexpr float SHIFT = !F32 && !BF ? 14.0f : 0.0f;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ long long before[PA_STRETCHES];
+    __shared__ long long warp_total[PA_WARPS];
+    __shared__ float part_m[PA_WARPS][2][PA_ROWS], part_l[PA_WARPS][2][PA_ROWS];
+    __shared__ int4 part_of[PA_WARPS][2];                                        // request, virtual head, 1 begins + 2 ends there, 1 (0: none)
+
+    const Shape s = p.s;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int rows_kept = min(s.group, PA_ROWS);
+    unsigned char *ring = smem + w * (PA_STAGES * 2 * PA_TILE);
+    float *first_part = reinterpret_cast<float *>(smem + PA_WARPS * PA_STAGES * 2 * PA_TILE) + w * rows_kept * HS;   // [rows][HS]
+    let_successor_start();
+    wait_for_predecessor();
+
+    // ---- how many tiles lie before each thread's stretch of requests ----
+    const int stretch = s.stretch();
+    long long mine = 0;
+    if (threadIdx.x < PA_STRETCHES)
+        for (int i = 0, r = threadIdx.x * stretch; i < stretch && r < s.n; ++i, ++r) mine += s.tiles(p.lens[r]);
+    long long sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += u;
     }
-    if (lane == 0) { m_of[w] = m; l_of[w] = l; }
-    for (int e = 0; e < E; ++e) o_of[w][lane * E + e] = o[e];
+    if (lane == 31) warp_total[w] = sum;
+    if (lane < 2) part_of[w][lane] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    float top = -INFINITY, all = 0.0f;
-    for (int j = 0; j < WARPS; ++j) top = fmaxf(top, m_of[j]);
-    for (int j = 0; j < WARPS; ++j) all += l_of[j] > 0.0f ? l_of[j] * expf(m_of[j] - top) : l_of[j];
-    for (int d = threadIdx.x; d < HS; d += blockDim.x) {
-        float x = 0.0f;
-        for (int j = 0; j < WARPS; ++j) if (l_of[j] != 0.0f) x += o_of[j][d] * expf(m_of[j] - top);
-        out[i * out_stride + h * HS + d] = all == 0.0f ? 0.0f : x / all;
+    long long total = 0;
+    for (int i = 0; i < PA_WARPS; ++i) {
+        if (i < w) sum += warp_total[i];
+        total += warp_total[i];
     }
-    if (lse && threadIdx.x == 0) lse[(size_t)i * heads + h] = all == 0.0f ? -INFINITY : top + logf(all);
+    if (threadIdx.x < PA_STRETCHES) before[threadIdx.x] = sum - mine;
+    __syncthreads();
+
+    const Line line(total * s.vheads, gridDim.x * PA_WARPS);
+    const int run = blockIdx.x * PA_WARPS + w;
+    if (total > 0 && run < line.warps) {
+        const long long t0 = line.begin(run);
+        const int count = (int)(line.begin(run + 1) - t0);
+        // the stretch that holds tile t0: the last one with no more tiles before it
+        int at = 0;
+        for (int i = lane; i < PA_STRETCHES; i += 32) at += __popc(__ballot_sync(0xffffffffu, before[i] * s.vheads <= t0 && (long long)i * stretch < s.n));
+        Place load;
+        load.set(s, p.lens, (at - 1) * stretch, t0 - before[at - 1] * s.vheads);
+        Place here = load;
+        // ---- the ring ----
+        constexpr int HELD = (KEYS + 31) / 32;
+        int page[HELD];                                       // of the rows that this lane looks up, for the tile that is loaded next
+        auto look_up = [&]() {
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                const unsigned key = (unsigned)load.tile * KEYS + i * 32 + lane;
+                page[i] = (KEYS >= 32 || lane < KEYS) && key < (unsigned)load.len ? p.tables[(size_t)load.request * p.max_pages + key / (unsigned)p.c.page_size] : -1;
+            }
+        };
+        unsigned valid[PA_STAGES][HELD];                      // rows that count, of each slot
+        auto start_load = [&](int slot) {
+            long long off[HELD];
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                const unsigned key = (unsigned)load.tile * KEYS + i * 32 + lane;
+                const bool ok = page[i] >= 0 && page[i] < p.c.pages;
+                off[i] = ok ? page[i] * p.c.page_stride + (key % (unsigned)p.c.page_size) * p.c.token_stride + (load.vhead / s.parts) * p.c.head_stride : -1;
+                const unsigned rows = __ballot_sync(0xffffffffu, ok);
+#pragma unroll
+                for (int j = 0; j < PA_STAGES; ++j)
+                    if (j == slot) valid[j][i] = rows;
+            }
+            unsigned char *k = ring + slot * 2 * PA_TILE, *v = k + PA_TILE;
+#pragma unroll
+            for (int i = 0; i < PA_TILE / 512; ++i) {
+                const int lin = i * 32 + lane, row = lin / UNITS, u = lin % UNITS;
+                const long long from = HELD == 1 ? __shfl_sync(0xffffffffu, off[0], row)
+                                                 : __shfl_sync(0xffffffffu, off[i * 32 / UNITS / 32], row & 31);
+                const int place = F32 ? fm::unit_of(row, u) : UNITS >= 8 ? u ^ (row & 7) : u ^ ((row >> 1) & 3);
+                const long long el = from < 0 ? 0 : from + u * (16 / (int)sizeof(T));
+                fm::cp_async16(k + (row * UNITS + place) * 16, (const T *)p.c.k + el, from >= 0);
+                fm::cp_async16(v + (row * UNITS + place) * 16, (const T *)p.c.v + el, from >= 0);
+            }
+            load.next(s, p.lens);
+        };
+        look_up();
+#pragma unroll
+        for (int i = 0; i < PA_STAGES - 1; ++i) {
+            if (i < count) {
+                start_load(i);
+                if (i + 1 < count) look_up();
+            }
+            fm::cp_commit();
+        }
+
+        // ---- the head at hand ----
+        // pieces of its queries: 16-bit types [HS / 16][first piece, second] (+ third for bf16), fp32 [HS / 8][4]
+        uint32_t qa[F32 ? 1 : HS / 16][4], ql[BF ? HS / 16 : 1][2];
+        float qf[F32 ? HS / 8 : 1][4];
+        float o[HS / 8][2], m = 0.0f, l = 0.0f, f = 0.0f;     // m in units of the scores as the products give them, f: log2's of one of those
+        bool begins = false;
+        int done = 0;                                         // parts kept for joining
+        auto begin_head = [&]() {
+            const int kept = min(PA_ROWS, s.group - (here.vhead % s.parts) * PA_ROWS);
+            const float *q = p.q + here.request * p.q_stride + (long long)((here.vhead / s.parts) * s.group + (here.vhead % s.parts) * PA_ROWS + g) * HS;
+            const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+            f = fabsf(p.scale) * 1.4426950408889634f;
+            if constexpr (F32) {
+#pragma unroll
+                for (int j = 0; j < HS / 16; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = g < kept ? q[16 * j + 4 * t + e] * sign : 0.0f, hi = round_tf32_alu(x);
+                        qf[2 * j + e / 2][(e & 1) * 2] = hi;
+                        qf[2 * j + e / 2][(e & 1) * 2 + 1] = x - hi;
+                    }
+            } else {
+                float x[HS / 16][4], top = 0.0f;
+#pragma unroll
+                for (int j = 0; j < HS / 16; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[j][e] = g < kept ? q[16 * j + 2 * t + (e & 1) + (e >> 1) * 8] * sign : 0.0f;
+                        top = fmaxf(top, fabsf(x[j][e]));
+                    }
+                if (!BF) {
+                    // the row's largest element to [2^14, 2^15)
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const int up = top > 0.0f && top < INFINITY ? min(14 - ilogbf(top), 126) : 0;
+                    const float by = ldexpf(1.0f, up);
+                    f = ldexpf(f, -up);
+#pragma unroll
+                    for (int j = 0; j < HS / 16; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[j][e] *= by;
+                }
+#pragma unroll
+                for (int j = 0; j < HS / 16; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t piece[BF ? 3 : 2];
+                        split<T>(x[j][2 * e], x[j][2 * e + 1], piece);
+                        qa[j][2 * e] = piece[0];
+                        qa[j][2 * e + 1] = piece[1];
+                        if (BF) ql[j][e] = piece[BF ? 2 : 0];
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < HS / 8; ++i) o[i][0] = o[i][1] = 0.0f;
+            m = -INFINITY;
+            l = 0.0f;
+            begins = here.tile == 0;
+        };
+        // element i, e of a lane's outputs: its column
+        auto column = [&](int i, int e) { return F32 ? (i / 4) * 32 + 8 * t + i % 4 + 4 * e : 8 * i + 2 * t + e; };
+        auto end_head = [&](bool ends) {
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            constexpr float down = !F32 && !BF ? 1.0f / 16384.0f : 1.0f;
+            const float top = m * f;                          // (-inf where nothing counted; f may be 0)
+            const int kept = min(PA_ROWS, s.group - (here.vhead % s.parts) * PA_ROWS);
+            l *= down;
+            if (begins && ends) {
+                if (g >= kept) return;
+                const int h = (here.vhead / s.parts) * s.group + (here.vhead % s.parts) * PA_ROWS + g;
+                float *to = p.out + here.request * p.out_stride + (long long)h * HS;
+                const float by = l == 0.0f ? 0.0f : down / l;
+#pragma unroll
+                for (int i = 0; i < HS / 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) to[column(i, e)] = o[i][e] * by;
+                if (p.lse && t == 0) p.lse[(size_t)here.request * s.heads + h] = l == 0.0f ? -INFINITY : fmaf(top, 0.6931471805599453f, logf(l));
+                return;
+            }
+            float *to = done == 0 ? first_part : reinterpret_cast<float *>(ring);
+            if (done == 1) {                                  // (the run's last head: nothing is in flight any more)
+                fm::cp_wait_all();
+                __syncwarp();
+            }
+            if (g < kept) {
+#pragma unroll
+                for (int i = 0; i < HS / 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) to[g * HS + column(i, e)] = o[i][e] * down;
+                if (t == 0) {
+                    part_m[w][done][g] = l == 0.0f ? -INFINITY : top;
+                    part_l[w][done][g] = l;
+                }
+            }
+            if (lane == 0) part_of[w][done] = make_int4(here.request, here.vhead, (begins ? 1 : 0) | (ends ? 2 : 0), 1);
+            ++done;
+        };
+
+        begin_head();
+        int slot = 0;
+        for (int j = 0; j < count; ++j) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(PA_STAGES - 2) : "memory");
+            __syncwarp();
+            if (j + PA_STAGES - 1 < count) {
+                start_load(slot == 0 ? PA_STAGES - 1 : slot - 1);
+                if (j + PA_STAGES < count) look_up();
+            }
+            fm::cp_commit();
+            unsigned rows[HELD];
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                rows[i] = valid[0][i];
+#pragma unroll
+                for (int k = 1; k < PA_STAGES; ++k)
+                    if (k == slot) rows[i] = valid[k][i];
+            }
+            const unsigned char *kt = ring + slot * 2 * PA_TILE, *vt = kt + PA_TILE;
+            const uint32_t ka = (uint32_t)__cvta_generic_to_shared(kt), va = ka + PA_TILE;
+            if (++slot == PA_STAGES) slot = 0;
+
+            // scores: keys 8 i + 2 t + e of row g
+            float sc[NT][2];
+            if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    float c[2][4] = {}, d[2][4] = {};
+#pragma unroll
+                    for (int jj = 0; jj < HS / 16; ++jj) {
+                        const float4 x = fm::tile_ld<HS>(reinterpret_cast<const float *>(kt), 8 * i + g, 4 * jj + t);
+                        const float4 h = make_float4(round_tf32_alu(x.x), round_tf32_alu(x.y), round_tf32_alu(x.z), round_tf32_alu(x.w));
+                        mma8(c[0], qf[2 * jj], h.x, h.y);
+                        mma8(c[1], qf[2 * jj + 1], h.z, h.w);
+                        mma8(d[0], qf[2 * jj], x.x - h.x, x.y - h.y);
+                        mma8(d[1], qf[2 * jj + 1], x.z - h.z, x.w - h.w);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) sc[i][e] = (c[0][e] + c[1][e]) + ((c[0][2 + e] + c[1][2 + e]) + (d[0][e] + d[1][e]));
+                }
+            } else {
+                const int id = lane >> 3;
+#pragma unroll
+                for (int i = 0; i < NT; i += 2) {
+                    float c[2][2][4] = {}, d[2][4] = {};
+                    const int row = 8 * i + (lane & 7) + (id >> 1) * 8;
+#pragma unroll
+                    for (int jj = 0; jj < HS / 16; ++jj) {
+                        const int u = 2 * jj + (id & 1);
+                        uint32_t b[4];
+                        ldmatrix4<false>(b, ka + (row * UNITS + (UNITS >= 8 ? u ^ (row & 7) : u ^ ((row >> 1) & 3))) * 16);
+                        mma16(c[0][jj & 1], qa[jj][0], qa[jj][1], qa[jj][2], qa[jj][3], b[0], b[1], T());
+                        mma16(c[1][jj & 1], qa[jj][0], qa[jj][1], qa[jj][2], qa[jj][3], b[2], b[3], T());
+                        if constexpr (BF) {
+                            mma16(d[0], ql[jj][0], 0, ql[jj][1], 0, b[0], b[1], T());
+                            mma16(d[1], ql[jj][0], 0, ql[jj][1], 0, b[2], b[3], T());
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) sc[i + k][e] = (c[k][0][e] + c[k][1][e]) + ((c[k][0][2 + e] + c[k][1][2 + e]) + d[k][e]);
+                }
+            }
+            // weights
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (rows[i / 4] >> (8 * (i % 4) + 2 * t + e) & 1) top = fmaxf(top, sc[i][e]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if (__any_sync(0xffffffffu, top > m)) {
+                const float mn = fmaxf(m, top), by = m == -INFINITY ? 0.0f : exp2f((m - mn) * f);
+                l *= by;
+#pragma unroll
+                for (int i = 0; i < HS / 8; ++i) { o[i][0] *= by; o[i][1] *= by; }
+                m = mn;
+            }
+            const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    sc[i][e] = rows[i / 4] >> (8 * (i % 4) + 2 * t + e) & 1 ? exp2f(fmaf(sc[i][e] - from, f, SHIFT)) : 0.0f;
+                    l += sc[i][e];
+                }
+            // weights times values
+            if constexpr (F32) {
+                float pw[NT][4];
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        pw[i][2 * e] = round_tf32_alu(sc[i][e]);
+                        pw[i][2 * e + 1] = sc[i][e] - pw[i][2 * e];
+                    }
+#pragma unroll
+                for (int d = 0; d < HS / 32; ++d) {
+                    float c[4][4] = {};
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        const float4 x = fm::tile_ld<HS>(reinterpret_cast<const float *>(vt), 8 * i + 2 * t, 8 * d + g);
+                        const float4 y = fm::tile_ld<HS>(reinterpret_cast<const float *>(vt), 8 * i + 2 * t + 1, 8 * d + g);
+                        const float a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float ah = round_tf32_alu(a[e]), bh = round_tf32_alu(b[e]);
+                            mma8(c[e], pw[i], ah, bh);
+                            mma8(c[e], pw[i], a[e] - ah, b[e] - bh);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) o[4 * d + e][k] += c[e][k] + c[e][2 + k];
+                }
+            } else {
+                uint32_t pw[NT][BF ? 3 : 2];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) split<T>(sc[i][0], sc[i][1], pw[i]);
+                const int id = lane >> 3;
+#pragma unroll
+                for (int d = 0; d < HS / 16; ++d) {
+                    float c[2][4] = {};
+#pragma unroll
+                    for (int i = 0; i < NT; i += 2) {
+                        const int row = 8 * i + (lane & 7) + (id & 1) * 8, u = 2 * d + (id >> 1);
+                        uint32_t b[4];
+                        ldmatrix4<true>(b, va + (row * UNITS + (UNITS >= 8 ? u ^ (row & 7) : u ^ ((row >> 1) & 3))) * 16);
+                        mma16(c[0], pw[i][0], pw[i][1], pw[i + 1][0], pw[i + 1][1], b[0], b[1], T());
+                        mma16(c[1], pw[i][0], pw[i][1], pw[i + 1][0], pw[i + 1][1], b[2], b[3], T());
+                        if constexpr (BF) {
+                            mma16(c[0], pw[i][2], 0, pw[i + 1][2], 0, b[0], b[1], T());
+                            mma16(c[1], pw[i][2], 0, pw[i + 1][2], 0, b[2], b[3], T());
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) o[2 * d + k][e] += c[k][e] + c[k][2 + e];
+                }
+            }
+            const bool ends = here.tile + 1 == here.tiles;
+            if (ends || j + 1 == count) {
+                end_head(ends);
+                if (j + 1 < count) {
+                    here.next(s, p.lens);
+                    begin_head();
+                }
+            } else {
+                ++here.tile;
+            }
+        }
+    }
+
+    // ---- heads that several of the block's warps, or blocks, have parts of ----
+    __syncthreads();
+    if (threadIdx.x == 0) p.w.begun[blockIdx.x] = make_int4(0, 0, 0, 0);
+    for (int e = 0; e < 2 * PA_WARPS;) {
+        const int4 of = part_of[e >> 1][e & 1];
+        if (!of.w) { ++e; continue; }
+        int last = e, flags = of.z;                           // entries [e, last] are parts of this head (or none)
+        for (int i = e + 1; i < 2 * PA_WARPS; ++i) {
+            const int4 x = part_of[i >> 1][i & 1];
+            if (!x.w) continue;
+            if (x.x != of.x || x.y != of.y) break;
+            last = i;
+            flags |= x.z;
+        }
+        const int kept = min(PA_ROWS, s.group - (of.y % s.parts) * PA_ROWS), slot = flags & 1;
+        for (int i = threadIdx.x; i < kept * HS; i += PA_THREADS) {
+            const int r = i / HS, d = i % HS;
+            float top = -INFINITY, all = 0.0f, x = 0.0f;
+            for (int k = e; k <= last; ++k)
+                if (part_of[k >> 1][k & 1].w) top = fmaxf(top, part_m[k >> 1][k & 1][r]);
+            for (int k = e; k <= last; ++k) {
+                if (!part_of[k >> 1][k & 1].w) continue;
+                const float pl = part_l[k >> 1][k & 1][r];
+                if (pl == 0.0f) continue;
+                const float by = exp2f(part_m[k >> 1][k & 1][r] - top);
+                const float *from = k & 1 ? reinterpret_cast<const float *>(smem + (k >> 1) * (PA_STAGES * 2 * PA_TILE))
+                                          : reinterpret_cast<const float *>(smem + PA_WARPS * PA_STAGES * 2 * PA_TILE) + (k >> 1) * rows_kept * HS;
+                all += pl * by;
+                x += from[r * HS + d] * by;
+            }
+            if (flags == 3) {
+                const int h = (of.y / s.parts) * s.group + (of.y % s.parts) * PA_ROWS + r;
+                p.out[of.x * p.out_stride + (long long)h * HS + d] = all == 0.0f ? 0.0f : x / all;
+                if (p.lse && d == 0) p.lse[(size_t)of.x * s.heads + h] = all == 0.0f ? -INFINITY : fmaf(top, 0.6931471805599453f, logf(all));
+            } else {
+                const size_t row = ((size_t)blockIdx.x * 2 + slot) * PA_ROWS + r;
+                p.w.o[row * HS + d] = x;
+                if (d == 0) {
+                    p.w.m[row] = top;
+                    p.w.l[row] = all;
+                }
+            }
+        }
+        if (flags == 1 && threadIdx.x == 0) {
+            // the head's last tile is in the run of another block
+            const int first = of.x / stretch * stretch;
+            const long long tile = s.last_tile(p.lens, of.x, of.y, first, before[of.x / stretch]);
+            p.w.begun[blockIdx.x] = make_int4(of.x, of.y, line.warp_of(tile) / PA_WARPS, 1);
+        }
+        e = last + 1;
+    }
+    // ---- requests without tokens ----
+    for (int r = blockIdx.x; r < s.n; r += gridDim.x) {
+        if (s.length(p.lens[r]) > 0) continue;
+        for (int i = threadIdx.x; i < s.heads * HS; i += PA_THREADS) p.out[r * p.out_stride + i] = 0.0f;
+        if (p.lse)
+            for (int h = threadIdx.x; h < s.heads; h += PA_THREADS) p.lse[(size_t)r * s.heads + h] = -INFINITY;
+    }
+}
+
+// The heads that reach over blocks: a block for each block of attend_k that began one, and each row.
+template <int HS>
+__global__ void __launch_bounds__(PA_THREADS) attend_join_k(const __grid_constant__ Attend p) {
+    constexpr int ACROSS = PA_THREADS / HS;
+    __shared__ float by[1024], red[32], sum[ACROSS][HS];
+    const Shape s = p.s;
+    const int r = blockIdx.y, d = threadIdx.x % HS, a = threadIdx.x / HS;
+    wait_for_predecessor();
+    const int4 of = p.w.begun[blockIdx.x];
+    if (!of.w || r >= min(PA_ROWS, s.group - (of.y % s.parts) * PA_ROWS)) return;
+    const int b0 = blockIdx.x, n = of.z - b0 + 1;             // parts: the second of block b0, the first of those behind it
+    auto row = [&](int i) { return ((size_t)(b0 + i) * 2 + (i == 0 ? 1 : 0)) * PA_ROWS + r; };
+    float top = -INFINITY;
+    for (int i = threadIdx.x; i < n; i += PA_THREADS) top = fmaxf(top, p.w.m[row(i)]);
+    // (a maximum of -inf, which block_reduce raises to the lowest number, has no weights: l is 0 throughout)
+    top = block_reduce<true>(top, red);
+    float all = 0.0f;
+    for (int i = threadIdx.x; i < n; i += PA_THREADS) {
+        const float l = p.w.l[row(i)], x = l == 0.0f ? 0.0f : exp2f(p.w.m[row(i)] - top);
+        by[i] = x;
+        all += l * x;
+    }
+    all = block_reduce<false>(all, red);                      // (its barriers also publish the weights)
+    float x = 0.0f;
+    for (int i = a; i < n; i += ACROSS) x += p.w.o[row(i) * HS + d] * by[i];
+    sum[a][d] = x;
+    __syncthreads();
+    if (a == 0) {
+#pragma unroll
+        for (int i = 1; i < ACROSS; ++i) x += sum[i][d];
+        const int h = (of.y / s.parts) * s.group + (of.y % s.parts) * PA_ROWS + r;
+        p.out[of.x * p.out_stride + (long long)h * HS + d] = all == 0.0f ? 0.0f : x / all;
+        if (p.lse && d == 0) p.lse[(size_t)of.x * s.heads + h] = all == 0.0f ? -INFINITY : fmaf(top, 0.6931471805599453f, logf(all));
+    }
 }
 
 size_t element(int type) { return type == BMB_TYPE_FP32 ? 4 : 2; }
@@ -84,13 +627,33 @@ int check_cache(const char *what, const bmb_kv_cache *c) {
     return BMB_OK;
 }
 
+Shape attend_shape(int n, int heads, int kv_heads, int hs, int type, int cap) {
+    Shape s;
+    s.n = n;
+    s.heads = heads;
+    s.group = heads / kv_heads;
+    s.parts = ceil_div(s.group, PA_ROWS);
+    s.vheads = kv_heads * s.parts;
+    s.cap = cap;
+    s.keys = PA_TILE / (hs * (int)element(type));
+    return s;
+}
+
+template <typename T, int HS>
+int run_attend(const Attend &p, cudaStream_t st) {
+    const int blocks = sm_count(), rows = p.s.group < PA_ROWS ? p.s.group : PA_ROWS;
+    const size_t smem = (size_t)PA_WARPS * (PA_STAGES * 2 * PA_TILE + rows * HS * sizeof(float));
+    BMB_CUDA(cudaFuncSetAttribute(attend_k<T, HS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  PA_WARPS * (PA_STAGES * 2 * PA_TILE + PA_ROWS * HS * (int)sizeof(float))));
+    BMB_TRY(launch_in_chain(attend_k<T, HS>, blocks, PA_THREADS, smem, st, p));
+    return launch_in_chain(attend_join_k<HS>, dim3(blocks, rows), PA_THREADS, 0, st, p);
+}
 template <typename T>
-int run_attend(float *out, float *lse, const float *q, const bmb_kv_cache &c, const int *tables, const int *lens, int n, int heads,
-               long long q_stride, long long out_stride, int max_pages, float scale, cudaStream_t st) {
-    switch (c.head_size) {
-    case 32: return launch(false, attend_k<T, 32>, n * heads, 256, 0, st, out, lse, q, c, tables, lens, heads, q_stride, out_stride, max_pages, scale);
-    case 64: return launch(false, attend_k<T, 64>, n * heads, 256, 0, st, out, lse, q, c, tables, lens, heads, q_stride, out_stride, max_pages, scale);
-    default: return launch(false, attend_k<T, 128>, n * heads, 256, 0, st, out, lse, q, c, tables, lens, heads, q_stride, out_stride, max_pages, scale);
+int run_attend(const Attend &p, cudaStream_t st) {
+    switch (p.c.head_size) {
+    case 32: return run_attend<T, 32>(p, st);
+    case 64: return run_attend<T, 64>(p, st);
+    default: return run_attend<T, 128>(p, st);
     }
 }
 
@@ -113,8 +676,61 @@ int bmb_paged_kv_write(const bmb_kv_cache *cache, const float *k, const float *v
 }
 
 size_t bmb_paged_attention_workspace(int heads, int kv_heads, int head_size) {
-    (void)heads; (void)kv_heads; (void)head_size;
-    return 16;
+    (void)heads;
+    (void)kv_heads;
+    return attend_workspace(sm_count(), head_size);
+}
+
+int bmb_paged_attention_schedule_check(const int *host_lens, int n, int heads, int kv_heads, int head_size, int type, int max_len, int blocks,
+                                       long long *tiles_out, int *joined_out) {
+    if (!host_lens || n <= 0 || kv_heads <= 0 || heads % kv_heads || max_len <= 0 || blocks <= 0 || type < BMB_TYPE_FP32 || type > BMB_TYPE_FP16 ||
+        (head_size != 32 && head_size != 64 && head_size != 128))
+        return fail(BMB_E_ARG, "paged_attention_schedule_check: bad argument");
+    const Shape s = attend_shape(n, heads, kv_heads, head_size, type, max_len);
+    long long total = 0;
+    std::vector<long long> before;                            // as a block counts them
+    for (int r = 0; r < n; ++r) {
+        if (r % s.stretch() == 0) before.push_back(total);
+        total += s.tiles(host_lens[r]);
+    }
+    const Line line(total * s.vheads, blocks * PA_WARPS);
+    long long tile = 0;
+    int joined = 0;
+    std::vector<int> goes_on(blocks, 0);                      // blocks that have a part of the head that an earlier block began
+    std::vector<int> promised(blocks, 0);
+    Place all{-1, s.vheads - 1, 0, 0, 0};                     // the line from its first tile to its last
+    for (int w = 0; total > 0 && w < line.warps; ++w) {
+        int at = 0, parts = 0;
+        while (at < (int)before.size() && before[at] * s.vheads <= line.begin(w)) ++at;
+        Place here;
+        here.set(s, host_lens, (at - 1) * s.stretch(), line.begin(w) - before[at - 1] * s.vheads);
+        bool begins = here.tile == 0;
+        for (long long j = line.begin(w); j < line.begin(w + 1); ++j, ++tile) {
+            all.next(s, host_lens);
+            if (j != tile || here.request >= n || here.request != all.request || here.vhead != all.vhead || here.tile != all.tile || line.warp_of(j) != w)
+                return fail(BMB_E_ARG, "paged_attention_schedule_check: warp %d has another tile at %lld", w, j);
+            const bool ends = here.tile + 1 == here.tiles, last = j + 1 == line.begin(w + 1);
+            if (!(ends || last)) { ++here.tile; continue; }
+            if (!(begins && ends) && ++parts > 2) return fail(BMB_E_ARG, "paged_attention_schedule_check: warp %d has %d parts", w, parts);
+            const int b = w / PA_WARPS;
+            const int end = line.warp_of(s.last_tile(host_lens, here.request, here.vhead, here.request / s.stretch() * s.stretch(), before[here.request / s.stretch()])) / PA_WARPS;
+            const int begin = line.warp_of(j - here.tile) / PA_WARPS;
+            if (begin < b) goes_on[b] = begin + 1;
+            if (begin == b && end > b) {
+                if (promised[b] != end) ++joined;
+                promised[b] = end;
+            }
+            here.next(s, host_lens);
+            begins = true;
+        }
+    }
+    if (tile != total * s.vheads) return fail(BMB_E_ARG, "paged_attention_schedule_check: %lld of %lld tiles", tile, total * s.vheads);
+    for (int b = 0; b < blocks; ++b)
+        for (int i = b + 1; i <= promised[b]; ++i)
+            if (goes_on[i] != b + 1) return fail(BMB_E_ARG, "paged_attention_schedule_check: block %d has no part of block %d's head", i, b);
+    if (tiles_out) *tiles_out = tile;
+    if (joined_out) *joined_out = joined;
+    return BMB_OK;
 }
 
 int bmb_paged_attention(float *out, float *lse, const float *q, const bmb_kv_cache *cache, const int *tables, const int *lens, int n, int heads,
@@ -132,12 +748,29 @@ int bmb_paged_attention(float *out, float *lse, const float *q, const bmb_kv_cac
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < bmb_paged_attention_workspace(heads, cache->heads, cache->head_size))
         return fail(BMB_E_ARG, "paged_attention: a workspace of %zu bytes, 16-byte aligned, is needed (got %zu)",
                     bmb_paged_attention_workspace(heads, cache->heads, cache->head_size), workspace_bytes);
+    Attend p{};
+    p.out = out;
+    p.lse = lse;
+    p.q = q;
+    p.c = *cache;
+    p.tables = tables;
+    p.lens = lens;
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    p.max_pages = max_pages;
+    p.scale = scale;
+    const int hs = cache->head_size, blocks = sm_count();
+    p.s = attend_shape(n, heads, cache->heads, hs, cache->type, max_pages * cache->page_size);
+    if ((double)n * p.s.vheads * p.s.tiles(p.s.cap) * blocks * PA_WARPS > 4e18)
+        return fail(BMB_E_LIMIT, "paged_attention: %d requests of %d tokens", n, p.s.cap);
+    p.w.o = (float *)workspace;
+    p.w.m = p.w.o + (size_t)blocks * 2 * PA_ROWS * hs;
+    p.w.l = p.w.m + (size_t)blocks * 2 * PA_ROWS;
+    p.w.begun = (int4 *)((char *)workspace + attend_workspace(blocks, hs) - (size_t)blocks * sizeof(int4));
     cudaStream_t st = (cudaStream_t)stream;
-    if (cache->type == BMB_TYPE_FP32)
-        return run_attend<float>(out, lse, q, *cache, tables, lens, n, heads, q_stride, out_stride, max_pages, scale, st);
-    if (cache->type == BMB_TYPE_BF16)
-        return run_attend<__nv_bfloat16>(out, lse, q, *cache, tables, lens, n, heads, q_stride, out_stride, max_pages, scale, st);
-    return run_attend<__half>(out, lse, q, *cache, tables, lens, n, heads, q_stride, out_stride, max_pages, scale, st);
+    if (cache->type == BMB_TYPE_FP32) return run_attend<float>(p, st);
+    if (cache->type == BMB_TYPE_BF16) return run_attend<__nv_bfloat16>(p, st);
+    return run_attend<__half>(p, st);
 }
 
 }  // extern "C"

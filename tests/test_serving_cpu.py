@@ -118,3 +118,25 @@ def test_oracle_assign_by_hand():
 def test_oracle_release_by_hand():
     stack, free, lens = serving_oracle.release(np.array([7, 2, 0, 0, 0, 0, 0, 0]), 2, [5, 4, 9], np.array([[5, -3, 1], [6, 9, 9], [3, 8, 4]]), [1, 0, 1], 4, 8)
     assert stack.tolist() == [7, 2, 5, 3, 4, 0, 0, 0] and free == 5 and lens.tolist() == [0, 4, 0]
+
+
+@pytest.mark.parametrize("blocks", [1, 2, 7, 148])
+@pytest.mark.parametrize("type_,hs", [(0, 128), (1, 32), (2, 64)])
+def test_every_tile_is_worked_on_once(bmb, blocks, type_, hs):
+    """The division of attention's work over warps and blocks, for lengths of all kinds."""
+    rng = np.random.default_rng(blocks + hs)
+    cases = [[0], [1], [5000], [0, 0, 0], [100000, 0, 1, 1], [1] * 500, [0] * 129 + [300], [300] + [0] * 700 + [2, 0], list(range(1, 260))]
+    cases += [list((rng.integers(0, 10 ** int(rng.integers(1, 5)), int(rng.integers(1, 700))) * (rng.random() < 0.9)).astype(int)) for _ in range(20)]
+    most = 0
+    for i, lens in enumerate(cases):
+        for heads, kv in ((1, 1), (6, 6), (32, 8), (71, 1), (24, 2)):
+            tiles, joined = C.c_longlong(), C.c_int()
+            a = np.array(lens, np.int32)
+            cap = 20000 if i % 5 else 10 ** 6
+            s = bmb.lib().bmb_paged_attention_schedule_check(a.ctypes.data, len(lens), heads, kv, hs, type_, cap, blocks, C.byref(tiles), C.byref(joined))
+            assert s == 0, bmb.lib().bmb_last_error()
+            keys = 4096 // (hs * (4 if type_ == 0 else 2))
+            assert tiles.value == sum(-(-min(max(int(x), 0), cap) // keys) for x in lens) * kv * -(-(heads // kv) // 8)
+            assert joined.value <= blocks
+            most = max(most, joined.value)
+    assert most > 0 or blocks == 1
