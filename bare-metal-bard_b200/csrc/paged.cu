@@ -2,6 +2,7 @@
 #include "flash_mma.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -46,44 +47,52 @@ __global__ void __launch_bounds__(256) kv_write_k(bmb_kv_cache c, const float *k
 // largest.  bf16: three of 8 bits, the third in an instruction of its own.  fp32: two TF32 pieces (fm, flash_mma.cuh) of queries and
 // weights, and of keys and values as they are read.  Sums over tiles are kept in fp32 registers.  Masked and absent tokens are zeros in
 // shared memory with a weight of zero, whatever the memory there holds.
-constexpr int PA_WARPS = 8, PA_THREADS = 32 * PA_WARPS, PA_STAGES = 3, PA_TILE = 4096, PA_ROWS = 8, PA_MIN_TILES = 1;
-constexpr int PA_STRETCHES = 128;       // stretches of requests whose tiles a block counts, to find where a run begins
+constexpr int PA_WARPS = 4, PA_THREADS = 32 * PA_WARPS, PA_STAGES = 3, PA_TILE = 4096, PA_ROWS = 8;
+constexpr int PA_BLOCKS = 2;            // blocks an SM
+constexpr int PA_MOST_BLOCKS = 1024;
+constexpr size_t PA_SMEM = 112 * 1024;   // dynamic shared memory with which two blocks fit an SM
 
-// All tiles in a line: requests in order, of each its (virtual) heads, of each its tiles.
+__host__ __device__ inline long long div_near(long long a, int b) { return a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b); }
+
+// All places in a line: requests in order, of each its (virtual) heads, of each its tiles and one place more, without work of its own, for
+// what a head costs to begin and to end (without it the runs with many short heads were the last to end: 9 heads in one of 11 tiles
+// took 31 us where the others took 24).
 struct Line {
-    long long tiles;
-    int warps;             // runs: warp w has tiles [begin(w), begin(w + 1))
-    __host__ __device__ Line(long long tiles_, int most) : tiles(tiles_), warps((int)(tiles_ / PA_MIN_TILES < most ? tiles_ / PA_MIN_TILES : most)) {
-        if (warps < 1) warps = 1;
+    long long places, each; // runs: warp w has places [begin(w), begin(w + 1)), `each` or one more
+    int warps, rest;
+    __host__ __device__ Line(long long places_, int most) : places(places_), warps((int)(places_ < most ? places_ > 1 ? places_ : 1 : most)) {
+        each = div_near(places, warps);
+        rest = (int)(places - each * warps);
     }
-    __host__ __device__ long long begin(int w) const { return tiles * w / warps; }
-    __host__ __device__ int warp_of(long long tile) const { return (int)(((tile + 1) * warps - 1) / tiles); }
+    __host__ __device__ long long begin(int w) const { return w * each + (w < rest ? w : rest); }
+    __host__ __device__ int warp_of(long long place) const {
+        const long long longer = rest * (each + 1);
+        return (int)(place < longer ? place / (each + 1) : rest + (place - longer) / each);
+    }
 };
 struct Shape {
-    int n, heads, group, parts, vheads, cap, keys;   // query heads a cache head, its groups of 8, virtual heads in all, longest length, keys a tile
+    int n, heads, group, parts, vheads, cap, keys_log2;   // query heads a cache head, its groups of 8, virtual heads in all, longest length, keys a tile
     __host__ __device__ int length(int len) const { return len < 0 ? 0 : len < cap ? len : cap; }
-    __host__ __device__ int stretch() const { return (n - 1) / PA_STRETCHES + 1; }
-    __host__ __device__ int tiles(int len) const { return (int)(((long long)length(len) + keys - 1) / keys); }
-    // the place in the line of a head's last tile; `before`: tiles (of one head each) of the requests before request `first`
-    __host__ __device__ long long last_tile(const int *lens, int request, int vhead, int first, long long before) const {
-        for (int i = first; i < request; ++i) before += tiles(lens[i]);
-        return before * vheads + (long long)(vhead + 1) * tiles(lens[request]) - 1;
-    }
+    __host__ __device__ int stretch() const { return (n - 1) / PA_THREADS + 1; }       // requests that a thread counts the tiles of
+    __host__ __device__ int places(int len) const { const int t = tiles(len); return t + (t > 0); }
+    __host__ __device__ int tiles(int len) const { return (int)(((unsigned)length(len) + (1u << keys_log2) - 1) >> keys_log2); }
 };
-// A place in the line.
+// A tile, and the request and virtual head that it is of.
 struct Place {
     int request, vhead, tile, tiles, len;
-    // to the tile `in` tiles behind the first one of request r
-    __host__ __device__ void set(const Shape &s, const int *lens, int r, long long in) {
-        for (; r + 1 < s.n && in >= (long long)s.tiles(lens[r]) * s.vheads; ++r) in -= (long long)s.tiles(lens[r]) * s.vheads;
+    // To the tile at the place `in` behind the first one of request r, or behind that place if it has none.  Places passed over (0 or 1).
+    __host__ __device__ int set(const Shape &s, const int *lens, int r, long long in) {
+        for (; r + 1 < s.n && in >= (long long)s.places(lens[r]) * s.vheads; ++r) in -= (long long)s.places(lens[r]) * s.vheads;
         request = r;
         len = s.length(lens[r]);
         tiles = s.tiles(len);
-        vhead = (int)(in / tiles);
-        tile = (int)(in % tiles);
+        vhead = (int)div_near(in, tiles + 1);
+        tile = (int)(in - (long long)vhead * (tiles + 1));
+        if (tile < tiles) return 0;
+        next_head(s, lens);
+        return 1;
     }
-    __host__ __device__ void next(const Shape &s, const int *lens) {
-        if (++tile < tiles) return;
+    __host__ __device__ void next_head(const Shape &s, const int *lens) {
         tile = 0;
         if (++vhead < s.vheads) return;
         vhead = 0;
@@ -91,6 +100,12 @@ struct Place {
             len = s.length(lens[request]);
             tiles = s.tiles(len);
         }
+    }
+    // to the next tile; how many places on it is (1 or 2)
+    __host__ __device__ int next(const Shape &s, const int *lens) {
+        if (++tile < tiles) return 1;
+        next_head(s, lens);
+        return 2;
     }
 };
 
@@ -143,6 +158,7 @@ struct Parts {
     int4 *begun;           // [blocks]: request, virtual head, last block, 1; or w = 0 where the block begins no head that others go on with
 };
 constexpr size_t part_floats(int blocks, int hs) { return (size_t)blocks * 2 * PA_ROWS * (hs + 2); }
+int attend_blocks() { return sm_count() * PA_BLOCKS < PA_MOST_BLOCKS ? sm_count() * PA_BLOCKS : PA_MOST_BLOCKS; }
 size_t attend_workspace(int blocks, int hs) { return (part_floats(blocks, hs) * sizeof(float) + 15) / 16 * 16 + (size_t)blocks * sizeof(int4); }
 
 struct Attend {
@@ -153,36 +169,42 @@ struct Attend {
     long long q_stride, out_stride;
     int max_pages;
     float scale;
+    bool staged, aligned_q;      // queries are staged in shared memory, 16 bytes at a time
     Shape s;
     Parts w;
 };
 
 template <typename T, int HS>
-__global__ void __launch_bounds__(PA_THREADS, 1) attend_k(const __grid_constant__ Attend p) {
+__global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant__ Attend p) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     constexpr int KEYS = PA_TILE / (HS * (int)sizeof(T)), NT = KEYS / 8;         // keys a tile, and tiles of 8
     constexpr int UNITS = HS * (int)sizeof(T) / 16;                              // 16-byte units of a row
     constexpr float SHIFT = !F32 && !BF ? 14.0f : 0.0f;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ long long before[PA_STRETCHES];
-    __shared__ long long warp_total[PA_WARPS];
+    __shared__ long long warp_total[PA_WARPS];                                   // (at the start)
     __shared__ float part_m[PA_WARPS][2][PA_ROWS], part_l[PA_WARPS][2][PA_ROWS];
     __shared__ int4 part_of[PA_WARPS][2];                                        // request, virtual head, 1 begins + 2 ends there, 1 (0: none)
+    __shared__ float weight[2 * PA_WARPS][PA_ROWS];
+    __shared__ int last_block[PA_WARPS + 1];                                      // that has a part of the head a warp has begun and not ended
+    int *group_of = reinterpret_cast<int *>(warp_total), &groups = last_block[PA_WARPS];      // first entry, last one << 8, what they say together << 16
+    static_assert(sizeof(warp_total) >= 2 * PA_WARPS * sizeof(int), "");
 
     const Shape s = p.s;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rows_kept = min(s.group, PA_ROWS);
     unsigned char *ring = smem + w * (PA_STAGES * 2 * PA_TILE);
+    // (of the dynamic memory: the rings, a part of a head for each warp, and before the first load how many places (of one head each) lie before each stretch)
+    long long *before = reinterpret_cast<long long *>(smem);
     float *first_part = reinterpret_cast<float *>(smem + PA_WARPS * PA_STAGES * 2 * PA_TILE) + w * rows_kept * HS;   // [rows][HS]
     let_successor_start();
     wait_for_predecessor();
 
-    // ---- how many tiles lie before each thread's stretch of requests ----
+    // ---- how many places (of one head each) lie before each thread's stretch of requests ----
     const int stretch = s.stretch();
     long long mine = 0;
-    if (threadIdx.x < PA_STRETCHES)
-        for (int i = 0, r = threadIdx.x * stretch; i < stretch && r < s.n; ++i, ++r) mine += s.tiles(p.lens[r]);
+    const int len_here = (int)blockIdx.x < s.n ? p.lens[blockIdx.x] : 1;
+    for (int i = 0, r = threadIdx.x * stretch; i < stretch && r < s.n; ++i, ++r) mine += s.places(p.lens[r]);
     long long sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -197,32 +219,42 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attend_k(const __grid_constant_
         if (i < w) sum += warp_total[i];
         total += warp_total[i];
     }
-    if (threadIdx.x < PA_STRETCHES) before[threadIdx.x] = sum - mine;
+    before[threadIdx.x] = sum - mine;
     __syncthreads();
 
     const Line line(total * s.vheads, gridDim.x * PA_WARPS);
     const int run = blockIdx.x * PA_WARPS + w;
+    // the stretch that holds the run's first place: the last one with no more places before it
+    int at = 0;
+    for (int i = lane; i < PA_THREADS; i += 32)
+        at += __popc(__ballot_sync(0xffffffffu, before[i] * s.vheads <= line.begin(run) && (long long)i * stretch < s.n));
+    const long long before_run = before[at > 0 ? at - 1 : 0] * s.vheads;
+    __syncthreads();
     if (total > 0 && run < line.warps) {
-        const long long t0 = line.begin(run);
-        const int count = (int)(line.begin(run + 1) - t0);
-        // the stretch that holds tile t0: the last one with no more tiles before it
-        int at = 0;
-        for (int i = lane; i < PA_STRETCHES; i += 32) at += __popc(__ballot_sync(0xffffffffu, before[i] * s.vheads <= t0 && (long long)i * stretch < s.n));
-        Place load;
-        load.set(s, p.lens, (at - 1) * stretch, t0 - before[at - 1] * s.vheads);
-        Place here = load;
+        const long long begin = line.begin(run);
+        const int end = (int)(line.begin(run + 1) - begin);   // places of the run, from 0
+        Place here;
+        int at_place = here.set(s, p.lens, (at - 1) * stretch, begin - before_run);
+        Place load = here;                                    // the tile that is loaded next
+        int load_place = at_place;
+        // queries of the first row of a head
+        auto queries = [&](const Place &x) {
+            return p.q + x.request * p.q_stride + (long long)((x.vhead / s.parts) * s.group + (x.vhead % s.parts) * PA_ROWS) * HS;
+        };
         // ---- the ring ----
         constexpr int HELD = (KEYS + 31) / 32;
-        int page[HELD];                                       // of the rows that this lane looks up, for the tile that is loaded next
-        auto look_up = [&]() {
+        // pages of the rows that this lane looks up
+        auto look_up = [&](const Place &x, int (&page)[HELD]) {
 #pragma unroll
             for (int i = 0; i < HELD; ++i) {
-                const unsigned key = (unsigned)load.tile * KEYS + i * 32 + lane;
-                page[i] = (KEYS >= 32 || lane < KEYS) && key < (unsigned)load.len ? p.tables[(size_t)load.request * p.max_pages + key / (unsigned)p.c.page_size] : -1;
+                const unsigned key = (unsigned)x.tile * KEYS + i * 32 + lane;
+                page[i] = (KEYS >= 32 || lane < KEYS) && key < (unsigned)x.len ? p.tables[(size_t)x.request * p.max_pages + key / (unsigned)p.c.page_size] : -1;
             }
         };
         unsigned valid[PA_STAGES][HELD];                      // rows that count, of each slot
-        auto start_load = [&](int slot) {
+        int heads_loaded = 0, heads_read = 0;                 // the staging buffer that is next (of two)
+        float *staged_q = reinterpret_cast<float *>(smem + PA_WARPS * (PA_STAGES * 2 * PA_TILE + rows_kept * HS * (int)sizeof(float))) + w * 2 * rows_kept * HS;
+        auto start_load = [&](const int (&page)[HELD], int slot) {
             long long off[HELD];
 #pragma unroll
             for (int i = 0; i < HELD; ++i) {
@@ -245,18 +277,24 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attend_k(const __grid_constant_
                 fm::cp_async16(k + (row * UNITS + place) * 16, (const T *)p.c.k + el, from >= 0);
                 fm::cp_async16(v + (row * UNITS + place) * 16, (const T *)p.c.v + el, from >= 0);
             }
-            load.next(s, p.lens);
-        };
-        look_up();
-#pragma unroll
-        for (int i = 0; i < PA_STAGES - 1; ++i) {
-            if (i < count) {
-                start_load(i);
-                if (i + 1 < count) look_up();
+            // A head's queries come with its first tile, or, where there is no room for them, on their way to L2 ahead of the reading.  Two
+            // buffers: when this tile is loaded the head at hand has read its own, so only the next tile's may still have to be read.
+            if (load.tile == 0) {
+                const float *q = queries(load);
+                const int floats = min(PA_ROWS, s.group - (load.vhead % s.parts) * PA_ROWS) * HS;
+                if (p.staged) {
+                    float *to = staged_q + heads_loaded * rows_kept * HS;
+                    if (p.aligned_q)
+                        for (int i = lane * 4; i < floats; i += 128) fm::cp_async16(to + i, q + i, true);
+                    else
+                        for (int i = lane; i < floats; i += 32) fm::cp_async4(to + i, q + i, true);
+                    heads_loaded ^= 1;
+                } else if (lane * 32 < floats) {
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(q + lane * 32));
+                }
             }
-            fm::cp_commit();
-        }
-
+            load_place += load.next(s, p.lens);
+        };
         // ---- the head at hand ----
         // pieces of its queries: 16-bit types [HS / 16][first piece, second] (+ third for bf16), fp32 [HS / 8][4]
         uint32_t qa[F32 ? 1 : HS / 16][4], ql[BF ? HS / 16 : 1][2];
@@ -264,51 +302,47 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attend_k(const __grid_constant_
         float o[HS / 8][2], m = 0.0f, l = 0.0f, f = 0.0f;     // m in units of the scores as the products give them, f: log2's of one of those
         bool begins = false;
         int done = 0;                                         // parts kept for joining
-        auto begin_head = [&]() {
+        // (x: a lane's elements of q, read ahead of what else waits for memory)
+        auto read_queries = [&](const float *q, float (&x)[HS / 4]) {
             const int kept = min(PA_ROWS, s.group - (here.vhead % s.parts) * PA_ROWS);
-            const float *q = p.q + here.request * p.q_stride + (long long)((here.vhead / s.parts) * s.group + (here.vhead % s.parts) * PA_ROWS + g) * HS;
-            const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+            q += g * HS;
+#pragma unroll
+            for (int i = 0; i < HS / 4; ++i) x[i] = g < kept ? q[16 * (i / 4) + (F32 ? 4 * t + i % 4 : 2 * t + (i & 1) + (i >> 1 & 1) * 8)] : 0.0f;
+        };
+        auto begin_head = [&](float (&x)[HS / 4]) {
             f = fabsf(p.scale) * 1.4426950408889634f;
+            if (p.scale < 0.0f)
+#pragma unroll
+                for (int i = 0; i < HS / 4; ++i) x[i] = -x[i];
             if constexpr (F32) {
 #pragma unroll
-                for (int j = 0; j < HS / 16; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = g < kept ? q[16 * j + 4 * t + e] * sign : 0.0f, hi = round_tf32_alu(x);
-                        qf[2 * j + e / 2][(e & 1) * 2] = hi;
-                        qf[2 * j + e / 2][(e & 1) * 2 + 1] = x - hi;
-                    }
+                for (int i = 0; i < HS / 4; ++i) {
+                    const float hi = round_tf32_alu(x[i]);
+                    qf[i / 2][(i & 1) * 2] = hi;
+                    qf[i / 2][(i & 1) * 2 + 1] = x[i] - hi;
+                }
             } else {
-                float x[HS / 16][4], top = 0.0f;
-#pragma unroll
-                for (int j = 0; j < HS / 16; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[j][e] = g < kept ? q[16 * j + 2 * t + (e & 1) + (e >> 1) * 8] * sign : 0.0f;
-                        top = fmaxf(top, fabsf(x[j][e]));
-                    }
                 if (!BF) {
                     // the row's largest element to [2^14, 2^15)
+                    float top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < HS / 4; ++i) top = fmaxf(top, fabsf(x[i]));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     const int up = top > 0.0f && top < INFINITY ? min(14 - ilogbf(top), 126) : 0;
                     const float by = ldexpf(1.0f, up);
                     f = ldexpf(f, -up);
 #pragma unroll
-                    for (int j = 0; j < HS / 16; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[j][e] *= by;
+                    for (int i = 0; i < HS / 4; ++i) x[i] *= by;
                 }
 #pragma unroll
-                for (int j = 0; j < HS / 16; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        uint32_t piece[BF ? 3 : 2];
-                        split<T>(x[j][2 * e], x[j][2 * e + 1], piece);
-                        qa[j][2 * e] = piece[0];
-                        qa[j][2 * e + 1] = piece[1];
-                        if (BF) ql[j][e] = piece[BF ? 2 : 0];
-                    }
+                for (int i = 0; i < HS / 8; ++i) {
+                    uint32_t piece[BF ? 3 : 2];
+                    split<T>(x[2 * i], x[2 * i + 1], piece);
+                    qa[i / 2][2 * (i & 1)] = piece[0];
+                    qa[i / 2][2 * (i & 1) + 1] = piece[1];
+                    if (BF) ql[i / 2][i & 1] = piece[BF ? 2 : 0];
+                }
             }
 #pragma unroll
             for (int i = 0; i < HS / 8; ++i) o[i][0] = o[i][1] = 0.0f;
@@ -352,18 +386,42 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attend_k(const __grid_constant_
                     part_l[w][done][g] = l;
                 }
             }
-            if (lane == 0) part_of[w][done] = make_int4(here.request, here.vhead, (begins ? 1 : 0) | (ends ? 2 : 0), 1);
+            if (lane == 0) {
+                part_of[w][done] = make_int4(here.request, here.vhead, (begins ? 1 : 0) | (ends ? 2 : 0), 1);
+                if (begins) last_block[w] = line.warp_of(begin + at_place + here.tiles - 1 - here.tile) / PA_WARPS;
+            }
             ++done;
         };
 
-        begin_head();
+        int next_page[HELD];                                  // for the tile that is loaded next
+        if (at_place < end) {
+            float x[HS / 4];
+            read_queries(queries(here), x);
+            heads_read ^= here.tile == 0;                     // (its first tile brings them again)
+            int page[PA_STAGES - 1][HELD];
+            Place ahead = load;
+            int ahead_place = load_place;
+#pragma unroll
+            for (int i = 0; i < PA_STAGES - 1; ++i)
+                if (ahead_place < end) {
+                    look_up(ahead, page[i]);
+                    ahead_place += ahead.next(s, p.lens);
+                }
+#pragma unroll
+            for (int i = 0; i < PA_STAGES - 1; ++i) {
+                if (load_place < end) start_load(page[i], i);
+                fm::cp_commit();
+            }
+            if (load_place < end) look_up(load, next_page);
+            begin_head(x);
+        }
         int slot = 0;
-        for (int j = 0; j < count; ++j) {
+        while (at_place < end) {
             asm volatile("cp.async.wait_group %0;" ::"n"(PA_STAGES - 2) : "memory");
             __syncwarp();
-            if (j + PA_STAGES - 1 < count) {
-                start_load(slot == 0 ? PA_STAGES - 1 : slot - 1);
-                if (j + PA_STAGES < count) look_up();
+            if (load_place < end) {
+                start_load(next_page, slot == 0 ? PA_STAGES - 1 : slot - 1);
+                if (load_place < end) look_up(load, next_page);
             }
             fm::cp_commit();
             unsigned rows[HELD];
@@ -500,84 +558,108 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attend_k(const __grid_constant_
                         for (int e = 0; e < 2; ++e) o[2 * d + k][e] += c[k][e] + c[k][2 + e];
                 }
             }
-            const bool ends = here.tile + 1 == here.tiles;
-            if (ends || j + 1 == count) {
-                end_head(ends);
-                if (j + 1 < count) {
-                    here.next(s, p.lens);
-                    begin_head();
+            const bool ends = here.tile + 1 == here.tiles, last = at_place + (ends ? 2 : 1) >= end;
+            if (ends || last) end_head(ends);
+            at_place += here.next(s, p.lens);
+            if (ends && !last) {
+                // the queries staged with the tile that is next, which has to have come
+                if (p.staged) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(PA_STAGES - 2) : "memory");
+                    __syncwarp();
                 }
-            } else {
-                ++here.tile;
+                float x[HS / 4];
+                read_queries(p.staged ? staged_q + heads_read * rows_kept * HS : queries(here), x);
+                heads_read ^= 1;
+                begin_head(x);
             }
         }
     }
 
     // ---- heads that several of the block's warps, or blocks, have parts of ----
     __syncthreads();
-    if (threadIdx.x == 0) p.w.begun[blockIdx.x] = make_int4(0, 0, 0, 0);
-    for (int e = 0; e < 2 * PA_WARPS;) {
-        const int4 of = part_of[e >> 1][e & 1];
-        if (!of.w) { ++e; continue; }
-        int last = e, flags = of.z;                           // entries [e, last] are parts of this head (or none)
-        for (int i = e + 1; i < 2 * PA_WARPS; ++i) {
-            const int4 x = part_of[i >> 1][i & 1];
-            if (!x.w) continue;
-            if (x.x != of.x || x.y != of.y) break;
-            last = i;
-            flags |= x.z;
-        }
-        const int kept = min(PA_ROWS, s.group - (of.y % s.parts) * PA_ROWS), slot = flags & 1;
-        for (int i = threadIdx.x; i < kept * HS; i += PA_THREADS) {
-            const int r = i / HS, d = i % HS;
-            float top = -INFINITY, all = 0.0f, x = 0.0f;
-            for (int k = e; k <= last; ++k)
-                if (part_of[k >> 1][k & 1].w) top = fmaxf(top, part_m[k >> 1][k & 1][r]);
-            for (int k = e; k <= last; ++k) {
-                if (!part_of[k >> 1][k & 1].w) continue;
-                const float pl = part_l[k >> 1][k & 1][r];
-                if (pl == 0.0f) continue;
-                const float by = exp2f(part_m[k >> 1][k & 1][r] - top);
-                const float *from = k & 1 ? reinterpret_cast<const float *>(smem + (k >> 1) * (PA_STAGES * 2 * PA_TILE))
-                                          : reinterpret_cast<const float *>(smem + PA_WARPS * PA_STAGES * 2 * PA_TILE) + (k >> 1) * rows_kept * HS;
-                all += pl * by;
-                x += from[r * HS + d] * by;
+    // A group is a head's entries one behind the other.  Each entry's weight in its group, a thread for each row; and the groups.
+    static_assert(2 * PA_WARPS * PA_ROWS <= PA_THREADS && 2 * PA_WARPS <= 32, "");
+    auto entry = [&](int i) { return part_of[i >> 1][i & 1]; };
+    auto same = [](int4 a, int4 b) { return a.w && b.w && a.x == b.x && a.y == b.y; };
+    if (threadIdx.x < 2 * PA_WARPS * PA_ROWS) {
+        const int e = threadIdx.x / PA_ROWS, r = threadIdx.x % PA_ROWS;
+        const int4 of = entry(e);
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 2 * PA_WARPS; ++i)
+            if (same(of, entry(i))) top = fmaxf(top, part_m[i >> 1][i & 1][r]);
+        const float l = part_l[e >> 1][e & 1][r];
+        // (NaN where the sum is: its maximum may be that of nothing)
+        weight[e][r] = !of.w || l == 0.0f ? 0.0f : l == l ? exp2f(part_m[e >> 1][e & 1][r] - top) : l;
+    } else if (w == PA_WARPS - 1) {
+        const int4 of = lane < 2 * PA_WARPS ? entry(lane) : make_int4(0, 0, 0, 0);
+        bool first = of.w;
+        int last = lane, flags = of.z;
+#pragma unroll
+        for (int i = 0; i < 2 * PA_WARPS; ++i)
+            if (same(of, entry(i))) {
+                if (i < lane) first = false;
+                if (i > lane) last = i;
+                flags |= entry(i).z;
             }
-            if (flags == 3) {
-                const int h = (of.y / s.parts) * s.group + (of.y % s.parts) * PA_ROWS + r;
-                p.out[of.x * p.out_stride + (long long)h * HS + d] = all == 0.0f ? 0.0f : x / all;
-                if (p.lse && d == 0) p.lse[(size_t)of.x * s.heads + h] = all == 0.0f ? -INFINITY : fmaf(top, 0.6931471805599453f, logf(all));
-            } else {
-                const size_t row = ((size_t)blockIdx.x * 2 + slot) * PA_ROWS + r;
-                p.w.o[row * HS + d] = x;
-                if (d == 0) {
-                    p.w.m[row] = top;
-                    p.w.l[row] = all;
-                }
+        const unsigned firsts = __ballot_sync(0xffffffffu, first);
+        if (first) group_of[__popc(firsts & ((1u << lane) - 1))] = lane | last << 8 | flags << 16;
+        if (first && flags == 1) p.w.begun[blockIdx.x] = make_int4(of.x, of.y, last_block[lane >> 1], 1);
+        if (lane == 0) groups = __popc(firsts);
+        if (!__any_sync(0xffffffffu, first && flags == 1) && lane == 0) p.w.begun[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < groups * rows_kept * (HS / 4); i += PA_THREADS) {
+        const int row_in = i / (HS / 4), d = i % (HS / 4) * 4, r = row_in % rows_kept;
+        const int gr = group_of[row_in / rows_kept], e0 = gr & 255, e1 = gr >> 8 & 255, flags = gr >> 16;
+        const int4 of = entry(e0);
+        const int h = (of.y / s.parts) * s.group + (of.y % s.parts) * PA_ROWS + r;
+        if (r >= s.group - (of.y % s.parts) * PA_ROWS) continue;
+        float all = 0.0f, top = -INFINITY, x[4] = {};
+#pragma unroll
+        for (int k = 0; k < 2 * PA_WARPS; ++k) {
+            const float by = k < e0 || k > e1 ? 0.0f : weight[k][r];      // (0 also for an entry between them that is none)
+            const float4 v = *reinterpret_cast<const float4 *>(
+                (k & 1 ? smem + (k >> 1) * (PA_STAGES * 2 * PA_TILE) : smem + PA_WARPS * PA_STAGES * 2 * PA_TILE + (k >> 1) * rows_kept * HS * sizeof(float)) +
+                (r * HS + d) * sizeof(float));
+            const bool use = by != 0.0f;
+            all = use ? fmaf(part_l[k >> 1][k & 1][r], by, all) : all;
+            top = use ? fmaxf(top, part_m[k >> 1][k & 1][r]) : top;
+            x[0] = use ? fmaf(v.x, by, x[0]) : x[0];
+            x[1] = use ? fmaf(v.y, by, x[1]) : x[1];
+            x[2] = use ? fmaf(v.z, by, x[2]) : x[2];
+            x[3] = use ? fmaf(v.w, by, x[3]) : x[3];
+        }
+        if (flags == 3) {
+            float *to = p.out + of.x * p.out_stride + (long long)h * HS + d;
+            const float by = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[j] = x[j] * by;
+            if (p.lse && d == 0) p.lse[(size_t)of.x * s.heads + h] = all == 0.0f ? -INFINITY : fmaf(top, 0.6931471805599453f, logf(all));
+        } else {
+            const size_t row = ((size_t)blockIdx.x * 2 + (flags & 1)) * PA_ROWS + r;
+            *reinterpret_cast<float4 *>(p.w.o + row * HS + d) = make_float4(x[0], x[1], x[2], x[3]);
+            if (d == 0) {
+                p.w.m[row] = top;
+                p.w.l[row] = all;
             }
         }
-        if (flags == 1 && threadIdx.x == 0) {
-            // the head's last tile is in the run of another block
-            const int first = of.x / stretch * stretch;
-            const long long tile = s.last_tile(p.lens, of.x, of.y, first, before[of.x / stretch]);
-            p.w.begun[blockIdx.x] = make_int4(of.x, of.y, line.warp_of(tile) / PA_WARPS, 1);
-        }
-        e = last + 1;
     }
     // ---- requests without tokens ----
     for (int r = blockIdx.x; r < s.n; r += gridDim.x) {
-        if (s.length(p.lens[r]) > 0) continue;
+        if (s.length(r == (int)blockIdx.x ? len_here : p.lens[r]) > 0) continue;
         for (int i = threadIdx.x; i < s.heads * HS; i += PA_THREADS) p.out[r * p.out_stride + i] = 0.0f;
         if (p.lse)
             for (int h = threadIdx.x; h < s.heads; h += PA_THREADS) p.lse[(size_t)r * s.heads + h] = -INFINITY;
     }
 }
 
+constexpr int PJ_THREADS = 256;
 // The heads that reach over blocks: a block for each block of attend_k that began one, and each row.
 template <int HS>
-__global__ void __launch_bounds__(PA_THREADS) attend_join_k(const __grid_constant__ Attend p) {
-    constexpr int ACROSS = PA_THREADS / HS;
-    __shared__ float by[1024], red[32], sum[ACROSS][HS];
+__global__ void __launch_bounds__(PJ_THREADS) attend_join_k(const __grid_constant__ Attend p) {
+    constexpr int ACROSS = PJ_THREADS / HS;
+    __shared__ float by[PA_MOST_BLOCKS], red[32], sum[ACROSS][HS];
     const Shape s = p.s;
     const int r = blockIdx.y, d = threadIdx.x % HS, a = threadIdx.x / HS;
     wait_for_predecessor();
@@ -586,11 +668,11 @@ __global__ void __launch_bounds__(PA_THREADS) attend_join_k(const __grid_constan
     const int b0 = blockIdx.x, n = of.z - b0 + 1;             // parts: the second of block b0, the first of those behind it
     auto row = [&](int i) { return ((size_t)(b0 + i) * 2 + (i == 0 ? 1 : 0)) * PA_ROWS + r; };
     float top = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += PA_THREADS) top = fmaxf(top, p.w.m[row(i)]);
+    for (int i = threadIdx.x; i < n; i += PJ_THREADS) top = fmaxf(top, p.w.m[row(i)]);
     // (a maximum of -inf, which block_reduce raises to the lowest number, has no weights: l is 0 throughout)
     top = block_reduce<true>(top, red);
     float all = 0.0f;
-    for (int i = threadIdx.x; i < n; i += PA_THREADS) {
+    for (int i = threadIdx.x; i < n; i += PJ_THREADS) {
         const float l = p.w.l[row(i)], x = l == 0.0f ? 0.0f : exp2f(p.w.m[row(i)] - top);
         by[i] = x;
         all += l * x;
@@ -635,21 +717,30 @@ Shape attend_shape(int n, int heads, int kv_heads, int hs, int type, int cap) {
     s.parts = ceil_div(s.group, PA_ROWS);
     s.vheads = kv_heads * s.parts;
     s.cap = cap;
-    s.keys = PA_TILE / (hs * (int)element(type));
+    s.keys_log2 = 0;
+    while ((PA_TILE >> s.keys_log2) > hs * (int)element(type)) ++s.keys_log2;
     return s;
 }
 
 template <typename T, int HS>
-int run_attend(const Attend &p, cudaStream_t st) {
-    const int blocks = sm_count(), rows = p.s.group < PA_ROWS ? p.s.group : PA_ROWS;
-    const size_t smem = (size_t)PA_WARPS * (PA_STAGES * 2 * PA_TILE + rows * HS * sizeof(float));
-    BMB_CUDA(cudaFuncSetAttribute(attend_k<T, HS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  PA_WARPS * (PA_STAGES * 2 * PA_TILE + PA_ROWS * HS * (int)sizeof(float))));
-    BMB_TRY(launch_in_chain(attend_k<T, HS>, blocks, PA_THREADS, smem, st, p));
-    return launch_in_chain(attend_join_k<HS>, dim3(blocks, rows), PA_THREADS, 0, st, p);
+int run_attend(Attend &p, cudaStream_t st) {
+    const int blocks = attend_blocks(), rows = p.s.group < PA_ROWS ? p.s.group : PA_ROWS;
+    // staged queries where two blocks still fit an SM (228 KB, of which a block takes 1 KB and the static 1.2 KB besides)
+    const size_t part = rows * HS * sizeof(float), least = (size_t)PA_WARPS * (PA_STAGES * 2 * PA_TILE + part);
+    p.staged = least + PA_WARPS * 2 * part <= PA_SMEM;
+    p.aligned_q = ((uintptr_t)p.q & 15) == 0 && p.q_stride % 4 == 0;
+    static std::atomic<unsigned long long> prepared{0};       // devices (those from 64 on are prepared every time)
+    const int dev = current_device();
+    const unsigned long long bit = dev >= 0 && dev < 64 ? 1ULL << dev : 0;
+    if (!(prepared.load(std::memory_order_relaxed) & bit)) {
+        BMB_CUDA(cudaFuncSetAttribute(attend_k<T, HS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PA_SMEM));
+        prepared.fetch_or(bit, std::memory_order_relaxed);
+    }
+    BMB_TRY(launch_in_chain(attend_k<T, HS>, blocks, PA_THREADS, least + (p.staged ? PA_WARPS * 2 * part : 0), st, p));
+    return launch_in_chain(attend_join_k<HS>, dim3(blocks, rows), PJ_THREADS, 0, st, p);
 }
 template <typename T>
-int run_attend(const Attend &p, cudaStream_t st) {
+int run_attend(Attend &p, cudaStream_t st) {
     switch (p.c.head_size) {
     case 32: return run_attend<T, 32>(p, st);
     case 64: return run_attend<T, 64>(p, st);
@@ -678,7 +769,7 @@ int bmb_paged_kv_write(const bmb_kv_cache *cache, const float *k, const float *v
 size_t bmb_paged_attention_workspace(int heads, int kv_heads, int head_size) {
     (void)heads;
     (void)kv_heads;
-    return attend_workspace(sm_count(), head_size);
+    return attend_workspace(attend_blocks(), head_size);
 }
 
 int bmb_paged_attention_schedule_check(const int *host_lens, int n, int heads, int kv_heads, int head_size, int type, int max_len, int blocks,
@@ -687,14 +778,14 @@ int bmb_paged_attention_schedule_check(const int *host_lens, int n, int heads, i
         (head_size != 32 && head_size != 64 && head_size != 128))
         return fail(BMB_E_ARG, "paged_attention_schedule_check: bad argument");
     const Shape s = attend_shape(n, heads, kv_heads, head_size, type, max_len);
-    long long total = 0;
+    long long total = 0, tiles = 0, done = 0;
     std::vector<long long> before;                            // as a block counts them
     for (int r = 0; r < n; ++r) {
         if (r % s.stretch() == 0) before.push_back(total);
-        total += s.tiles(host_lens[r]);
+        total += s.places(host_lens[r]);
+        tiles += (long long)s.tiles(host_lens[r]) * s.vheads;
     }
     const Line line(total * s.vheads, blocks * PA_WARPS);
-    long long tile = 0;
     int joined = 0;
     std::vector<int> goes_on(blocks, 0);                      // blocks that have a part of the head that an earlier block began
     std::vector<int> promised(blocks, 0);
@@ -703,32 +794,34 @@ int bmb_paged_attention_schedule_check(const int *host_lens, int n, int heads, i
         int at = 0, parts = 0;
         while (at < (int)before.size() && before[at] * s.vheads <= line.begin(w)) ++at;
         Place here;
-        here.set(s, host_lens, (at - 1) * s.stretch(), line.begin(w) - before[at - 1] * s.vheads);
+        const long long begin = line.begin(w), end = line.begin(w + 1);
+        long long place = begin + here.set(s, host_lens, (at - 1) * s.stretch(), begin - before[at - 1] * s.vheads);
         bool begins = here.tile == 0;
-        for (long long j = line.begin(w); j < line.begin(w + 1); ++j, ++tile) {
+        while (place < end) {
             all.next(s, host_lens);
-            if (j != tile || here.request >= n || here.request != all.request || here.vhead != all.vhead || here.tile != all.tile || line.warp_of(j) != w)
-                return fail(BMB_E_ARG, "paged_attention_schedule_check: warp %d has another tile at %lld", w, j);
-            const bool ends = here.tile + 1 == here.tiles, last = j + 1 == line.begin(w + 1);
-            if (!(ends || last)) { ++here.tile; continue; }
-            if (!(begins && ends) && ++parts > 2) return fail(BMB_E_ARG, "paged_attention_schedule_check: warp %d has %d parts", w, parts);
-            const int b = w / PA_WARPS;
-            const int end = line.warp_of(s.last_tile(host_lens, here.request, here.vhead, here.request / s.stretch() * s.stretch(), before[here.request / s.stretch()])) / PA_WARPS;
-            const int begin = line.warp_of(j - here.tile) / PA_WARPS;
-            if (begin < b) goes_on[b] = begin + 1;
-            if (begin == b && end > b) {
-                if (promised[b] != end) ++joined;
-                promised[b] = end;
+            ++done;
+            if (here.request >= n || here.request != all.request || here.vhead != all.vhead || here.tile != all.tile || line.warp_of(place) != w)
+                return fail(BMB_E_ARG, "paged_attention_schedule_check: warp %d has another tile at %lld", w, place);
+            const bool ends = here.tile + 1 == here.tiles, last = place + (ends ? 2 : 1) >= end;
+            if (ends || last) {
+                if (!(begins && ends) && ++parts > 2) return fail(BMB_E_ARG, "paged_attention_schedule_check: warp %d has %d parts", w, parts);
+                const int b = w / PA_WARPS, first_block = line.warp_of(place - here.tile) / PA_WARPS;
+                const int last_block = line.warp_of(place + here.tiles - 1 - here.tile) / PA_WARPS;
+                if (first_block < b) goes_on[b] = first_block + 1;
+                if (first_block == b && last_block > b) {
+                    if (promised[b] != last_block) ++joined;
+                    promised[b] = last_block;
+                }
+                begins = true;
             }
-            here.next(s, host_lens);
-            begins = true;
+            place += here.next(s, host_lens);
         }
     }
-    if (tile != total * s.vheads) return fail(BMB_E_ARG, "paged_attention_schedule_check: %lld of %lld tiles", tile, total * s.vheads);
+    if (done != tiles) return fail(BMB_E_ARG, "paged_attention_schedule_check: %lld of %lld tiles", done, tiles);
     for (int b = 0; b < blocks; ++b)
         for (int i = b + 1; i <= promised[b]; ++i)
             if (goes_on[i] != b + 1) return fail(BMB_E_ARG, "paged_attention_schedule_check: block %d has no part of block %d's head", i, b);
-    if (tiles_out) *tiles_out = tile;
+    if (tiles_out) *tiles_out = tiles;
     if (joined_out) *joined_out = joined;
     return BMB_OK;
 }
@@ -759,9 +852,9 @@ int bmb_paged_attention(float *out, float *lse, const float *q, const bmb_kv_cac
     p.out_stride = out_stride;
     p.max_pages = max_pages;
     p.scale = scale;
-    const int hs = cache->head_size, blocks = sm_count();
+    const int hs = cache->head_size, blocks = attend_blocks();
     p.s = attend_shape(n, heads, cache->heads, hs, cache->type, max_pages * cache->page_size);
-    if ((double)n * p.s.vheads * p.s.tiles(p.s.cap) * blocks * PA_WARPS > 4e18)
+    if ((double)n * p.s.vheads * p.s.places(p.s.cap) > 1e12)
         return fail(BMB_E_LIMIT, "paged_attention: %d requests of %d tokens", n, p.s.cap);
     p.w.o = (float *)workspace;
     p.w.m = p.w.o + (size_t)blocks * 2 * PA_ROWS * hs;
