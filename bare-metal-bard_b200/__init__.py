@@ -226,10 +226,15 @@ def ptr(t):
     return t.ctypes.data
 
 
+_PLAIN = frozenset((int, float, type(None), KvCache, LogitRules))      # what ctypes takes as it is
+
+
 def call(name, *args):
     """Call a status-returning entry point with tensors turned into pointers."""
-    conv = [ptr(a) if (a is None or hasattr(a, "data_ptr") or hasattr(a, "ctypes")) else a for a in args]
-    check(getattr(lib(), name)(*conv), name)
+    conv = [a if a.__class__ in _PLAIN or not (hasattr(a, "data_ptr") or hasattr(a, "ctypes")) else ptr(a) for a in args]
+    status = getattr(_lib or lib(), name)(*conv)
+    if status:
+        check(status, name)
 
 
 def paged_attention_workspace(heads, kv_heads, head_size):

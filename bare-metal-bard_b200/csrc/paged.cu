@@ -11,22 +11,55 @@
 namespace bmb {
 namespace {
 
+__host__ __device__ inline long long div_near(long long a, int b) { return a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b); }
+
 template <typename T> __device__ __forceinline__ T from_float(float x);
 template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
-template <typename T>
-__global__ void __launch_bounds__(256) kv_write_k(bmb_kv_cache c, const float *k, const float *v, long long row_stride, const int *slots) {
-    const int slot = slots[blockIdx.x];
-    if (slot < 0 || slot >= c.pages * c.page_size) return;
-    const long long page = slot / c.page_size, off = slot % c.page_size;
-    for (int e = threadIdx.x; e < c.heads * c.head_size; e += blockDim.x) {
-        const long long from = blockIdx.x * row_stride + e;
-        const long long to = page * c.page_stride + off * c.token_stride + (e / c.head_size) * c.head_stride + e % c.head_size;
-        ((T *)c.k)[to] = from_float<T>(k[from]);
-        ((T *)c.v)[to] = from_float<T>(v[from]);
+// Keys and values of new tokens into their slots: a thread takes 16 bytes of the cache, of keys and of values.  Bound by memory.  VEC: the
+// rows are 16-byte aligned.
+constexpr int KW_THREADS = 256;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(KW_THREADS) kv_write_k(const __grid_constant__ bmb_kv_cache c, const float *k, const float *v, long long row_stride, const int *slots,
+                                                         int tokens, int units) {
+    constexpr int E = 16 / (int)sizeof(T);                    // elements a unit; `units` of them a row
+    let_successor_start();
+    wait_for_predecessor();
+    const long long at = (long long)blockIdx.x * KW_THREADS + threadIdx.x;
+    const int token = (int)div_near(at, units), e = (int)(at - (long long)token * units) * E;
+    if (token >= tokens) return;
+    const int slot = slots[token];
+    float x[2][E];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float *from = (i ? v : k) + token * row_stride + e;
+#pragma unroll
+        for (int j = 0; j < E; j += VEC ? 4 : 1) {
+            if (VEC) *reinterpret_cast<float4 *>(&x[i][j]) = *reinterpret_cast<const float4 *>(from + j);
+            else x[i][j] = from[j];
+        }
     }
+    if (slot < 0 || slot >= c.pages * c.page_size) return;
+    const int page = slot / c.page_size, head = e / c.head_size;
+    const long long to = page * c.page_stride + (slot - page * c.page_size) * c.token_stride + head * c.head_stride + (e - head * c.head_size);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        alignas(16) T y[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) y[j] = from_float<T>(x[i][j]);
+        *reinterpret_cast<uint4 *>((T *)(i ? c.v : c.k) + to) = *reinterpret_cast<const uint4 *>(y);
+    }
+}
+
+template <typename T>
+int run_write(const bmb_kv_cache &c, const float *k, const float *v, long long row_stride, const int *slots, int tokens, cudaStream_t st) {
+    const int units = c.heads * c.head_size / (16 / (int)sizeof(T));
+    const long long blocks = ((long long)tokens * units + KW_THREADS - 1) / KW_THREADS;
+    if (blocks > INT_MAX) return fail(BMB_E_LIMIT, "paged_kv_write: %d tokens of %d heads", tokens, c.heads);
+    const bool vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && row_stride % 4 == 0;
+    return launch_in_chain(vec ? kv_write_k<T, true> : kv_write_k<T, false>, (unsigned)blocks, KW_THREADS, 0, st, c, k, v, row_stride, slots, tokens, units);
 }
 
 // ---- attention of one token of each request ---------------------------------------------------------------------------
@@ -49,10 +82,8 @@ __global__ void __launch_bounds__(256) kv_write_k(bmb_kv_cache c, const float *k
 // shared memory with a weight of zero, whatever the memory there holds.
 constexpr int PA_WARPS = 4, PA_THREADS = 32 * PA_WARPS, PA_STAGES = 3, PA_TILE = 4096, PA_ROWS = 8;
 constexpr int PA_BLOCKS = 2;            // blocks an SM
-constexpr int PA_MOST_BLOCKS = 1024;
+constexpr int PA_MOST_BLOCKS = 512;
 constexpr size_t PA_SMEM = 112 * 1024;   // dynamic shared memory with which two blocks fit an SM
-
-__host__ __device__ inline long long div_near(long long a, int b) { return a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b); }
 
 // All places in a line: requests in order, of each its (virtual) heads, of each its tiles and one place more, without work of its own, for
 // what a head costs to begin and to end (without it the runs with many short heads were the last to end: 9 heads in one of 11 tiles
@@ -654,40 +685,60 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
     }
 }
 
-constexpr int PJ_THREADS = 256;
-// The heads that reach over blocks: a block for each block of attend_k that began one, and each row.
+// The heads that reach over blocks: a block for each block of attend_k that began one, and each row.  Parts are read 16 to 64 at a
+// time and four of those ahead of the sums: with two at a time one head in 132 parts took 8 us.
+constexpr int PJ_THREADS = 512;
 template <int HS>
 __global__ void __launch_bounds__(PJ_THREADS) attend_join_k(const __grid_constant__ Attend p) {
-    constexpr int ACROSS = PJ_THREADS / HS;
+    constexpr int ACROSS = PJ_THREADS * 4 / HS, HELD = PA_MOST_BLOCKS / PJ_THREADS;
     __shared__ float by[PA_MOST_BLOCKS], red[32], sum[ACROSS][HS];
     const Shape s = p.s;
-    const int r = blockIdx.y, d = threadIdx.x % HS, a = threadIdx.x / HS;
+    const int r = blockIdx.y, d = threadIdx.x % (HS / 4) * 4, a = threadIdx.x / (HS / 4);
     wait_for_predecessor();
     const int4 of = p.w.begun[blockIdx.x];
     if (!of.w || r >= min(PA_ROWS, s.group - (of.y % s.parts) * PA_ROWS)) return;
     const int b0 = blockIdx.x, n = of.z - b0 + 1;             // parts: the second of block b0, the first of those behind it
     auto row = [&](int i) { return ((size_t)(b0 + i) * 2 + (i == 0 ? 1 : 0)) * PA_ROWS + r; };
-    float top = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += PJ_THREADS) top = fmaxf(top, p.w.m[row(i)]);
-    // (a maximum of -inf, which block_reduce raises to the lowest number, has no weights: l is 0 throughout)
+    float m[HELD], l[HELD], top = -INFINITY, all = 0.0f;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+        const int i = threadIdx.x + k * PJ_THREADS;
+        m[k] = i < n ? p.w.m[row(i)] : -INFINITY;
+        l[k] = i < n ? p.w.l[row(i)] : 0.0f;
+        top = fmaxf(top, m[k]);
+    }
+    // (a maximum of -inf, which block_reduce raises to the lowest number, has no weights: l is 0 throughout, or NaN)
     top = block_reduce<true>(top, red);
-    float all = 0.0f;
-    for (int i = threadIdx.x; i < n; i += PJ_THREADS) {
-        const float l = p.w.l[row(i)], x = l == 0.0f ? 0.0f : exp2f(p.w.m[row(i)] - top);
-        by[i] = x;
-        all += l * x;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+        const float x = l[k] == 0.0f ? 0.0f : exp2f(m[k] - top);
+        if (threadIdx.x + k * PJ_THREADS < n) by[threadIdx.x + k * PJ_THREADS] = x;
+        all += l[k] * x;
     }
     all = block_reduce<false>(all, red);                      // (its barriers also publish the weights)
-    float x = 0.0f;
-    for (int i = a; i < n; i += ACROSS) x += p.w.o[row(i) * HS + d] * by[i];
-    sum[a][d] = x;
-    __syncthreads();
-    if (a == 0) {
+    float x[4] = {};
+    for (int i = a; i < n; i += 4 * ACROSS) {
+        float4 v[4];
 #pragma unroll
-        for (int i = 1; i < ACROSS; ++i) x += sum[i][d];
+        for (int k = 0; k < 4; ++k) v[k] = i + k * ACROSS < n ? *reinterpret_cast<const float4 *>(p.w.o + row(i + k * ACROSS) * HS + d) : make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float w = i + k * ACROSS < n ? by[i + k * ACROSS] : 0.0f;
+            x[0] = fmaf(v[k].x, w, x[0]);
+            x[1] = fmaf(v[k].y, w, x[1]);
+            x[2] = fmaf(v[k].z, w, x[2]);
+            x[3] = fmaf(v[k].w, w, x[3]);
+        }
+    }
+    *reinterpret_cast<float4 *>(&sum[a][d]) = make_float4(x[0], x[1], x[2], x[3]);
+    __syncthreads();
+    if (threadIdx.x < HS) {
+        float y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ACROSS; ++i) y += sum[i][threadIdx.x];
         const int h = (of.y / s.parts) * s.group + (of.y % s.parts) * PA_ROWS + r;
-        p.out[of.x * p.out_stride + (long long)h * HS + d] = all == 0.0f ? 0.0f : x / all;
-        if (p.lse && d == 0) p.lse[(size_t)of.x * s.heads + h] = all == 0.0f ? -INFINITY : fmaf(top, 0.6931471805599453f, logf(all));
+        p.out[of.x * p.out_stride + (long long)h * HS + threadIdx.x] = all == 0.0f ? 0.0f : y / all;
+        if (p.lse && threadIdx.x == 0) p.lse[(size_t)of.x * s.heads + h] = all == 0.0f ? -INFINITY : fmaf(top, 0.6931471805599453f, logf(all));
     }
 }
 
@@ -700,6 +751,7 @@ int check_cache(const char *what, const bmb_kv_cache *c) {
         return fail(BMB_E_ARG, "%s: bad sizes (pages=%d page_size=%d heads=%d)", what, c->pages, c->page_size, c->heads);
     if (c->head_size != 32 && c->head_size != 64 && c->head_size != 128)
         return fail(BMB_E_UNSUPPORTED, "%s: head size %d (32, 64 and 128 are served)", what, c->head_size);
+    if ((long long)c->heads * c->head_size > INT_MAX) return fail(BMB_E_LIMIT, "%s: %d heads", what, c->heads);
     if ((long long)c->pages * c->page_size > INT_MAX) return fail(BMB_E_LIMIT, "%s: %d pages of %d tokens are beyond an int", what, c->pages, c->page_size);
     const long long unit = 16 / (long long)element(c->type);
     const long long strides[] = {c->page_stride, c->token_stride, c->head_stride};
@@ -761,9 +813,9 @@ int bmb_paged_kv_write(const bmb_kv_cache *cache, const float *k, const float *v
     if (tokens == 0) return BMB_OK;
     if (!k || !v || !slots || ((uintptr_t)k | (uintptr_t)v) & 3) return fail(BMB_E_ARG, "paged_kv_write: a null or unaligned pointer");
     cudaStream_t st = (cudaStream_t)stream;
-    if (cache->type == BMB_TYPE_FP32) return launch(false, kv_write_k<float>, tokens, 256, 0, st, *cache, k, v, row_stride, slots);
-    if (cache->type == BMB_TYPE_BF16) return launch(false, kv_write_k<__nv_bfloat16>, tokens, 256, 0, st, *cache, k, v, row_stride, slots);
-    return launch(false, kv_write_k<__half>, tokens, 256, 0, st, *cache, k, v, row_stride, slots);
+    if (cache->type == BMB_TYPE_FP32) return run_write<float>(*cache, k, v, row_stride, slots, tokens, st);
+    if (cache->type == BMB_TYPE_BF16) return run_write<__nv_bfloat16>(*cache, k, v, row_stride, slots, tokens, st);
+    return run_write<__half>(*cache, k, v, row_stride, slots, tokens, st);
 }
 
 size_t bmb_paged_attention_workspace(int heads, int kv_heads, int head_size) {

@@ -1,146 +1,234 @@
 // Pages of a cache that several requests share: handed out by the requests' lengths (bmb_pages_assign) and taken back
 // (bmb_pages_release), on the GPU, so that a step's shapes never have to come back to the host.
 //
-// Both are sums over requests in their order (where a request's tokens and pages begin) and stores that follow from them.
+// Both are sums over requests in their order (where a request's tokens and pages begin) and stores that follow from them.  What they
+// move is little, so what they take is the chain of loads: lengths, then pages.  A block counts a stretch of requests with a thread
+// each, and tokens (of assign) or table entries (of release) are then dealt to threads whatever requests they are of.  Few
+// of them: one block.  Many: a cluster of 8, each of which counts all of them, with the block number of tokens or entries divided over the
+// cluster; lengths are read by all before any is overwritten, which a cluster's barrier can say and a grid cannot.
 #include "common.cuh"
 #include <climits>
 
 namespace bmb {
 namespace {
 
-constexpr int PG_THREADS = 1024, PG_WARPS = PG_THREADS / 32;
+constexpr int PG_CLUSTER = 8, PG_MOST = 1024;
 
-// The sum over the threads before and including this one; `total`: of all of them. `warps` is shared.
-__device__ __forceinline__ long long block_scan(long long v, long long *warps, long long *total) {
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+template <int BLOCKS>
+__device__ __forceinline__ void sync_all() {
+    if (BLOCKS == 1) {
+        __syncthreads();
+    } else {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+}
+// *p of another block of the cluster
+__device__ __forceinline__ long long read_of(const long long *p, unsigned rank) {
+    long long v;
+    asm volatile("{\n.reg .u32 a;\nmapa.shared::cluster.u32 a, %1, %2;\nld.shared::cluster.s64 %0, [a];\n}" : "=l"(v) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank) : "memory");
+    return v;
+}
+
+// The sum over the threads before and including this one; `total`: of all of them.  `sums` (shared, one a warp) is free again after the
+// next barrier.
+template <int THREADS>
+__device__ __forceinline__ long long block_scan(long long v, long long *sums, long long *total) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
     }
+    if (lane == 31) sums[w] = v;
     __syncthreads();
-    if (lane == 31) warps[w] = v;
-    __syncthreads();
-    long long before = 0, all = 0;
-    for (int i = 0; i < PG_WARPS; ++i) {
-        if (i < w) before += warps[i];
-        all += warps[i];
+    long long s = lane < THREADS / 32 ? sums[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += u;
     }
-    *total = all;
-    return before + v;
+    *total = __shfl_sync(0xffffffffu, s, 31);
+    const long long before = __shfl_sync(0xffffffffu, s, w > 0 ? w - 1 : 0);
+    return v + (w > 0 ? before : 0);
 }
 
-__device__ __forceinline__ int pages_of(long long tokens, int page_size) { return (int)((tokens + page_size - 1) / page_size); }
+__device__ __forceinline__ int pages_of(int tokens, int page_size) { return (int)(((long long)tokens + page_size - 1) / page_size); }
 
-__global__ void __launch_bounds__(PG_THREADS) assign_k(int *tables, int *lens_out, int *slots, int *positions, int *owners, int *starts,
-                                                       int *free_left, const int *lens, const int *new_lens, const int *free_pages,
-                                                       const int *free_count, int n, int max_pages, int page_size, int pages, int max_tokens) {
-    __shared__ long long warps[PG_WARPS];
-    __shared__ long long begin_of[PG_THREADS], page_begin[PG_THREADS];
-    __shared__ int len_of[PG_THREADS], new_of[PG_THREADS], need_of[PG_THREADS];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+template <int BLOCKS, int THREADS>
+__global__ void __launch_bounds__(THREADS) assign_k(int *tables, int *lens_out, int *slots, int *positions, int *owners, int *starts,
+                                                    int *free_left, const int *lens, const int *new_lens, const int *free_pages,
+                                                    const int *free_count, int n, int max_pages, int page_size, int pages, int max_tokens) {
+    __shared__ long long sums[2][THREADS / 32];
+    // of the stretch's requests: where tokens and new pages begin, length, pages held (< 0: not served, ~held)
+    __shared__ int begin_of[THREADS], page_begin[THREADS], len_of[THREADS], held_of[THREADS];
+    __shared__ int taken;
+    const int me = BLOCKS == 1 ? 0 : (int)cluster_rank();
+    if (threadIdx.x == 0) taken = 0;
+    let_successor_start();
+    wait_for_predecessor();
     const int F = min(max(*free_count, 0), pages);
-    long long tokens_before = 0, pages_before = 0, taken = 0;
-    for (int base = 0; base < n; base += PG_THREADS) {
+    long long tokens_before = 0, pages_before = 0;
+    for (int base = 0; base < n; base += THREADS) {
         const int i = base + threadIdx.x;
         const int L = i < n ? max(lens[i], 0) : 0, A = i < n ? max(new_lens[i], 0) : 0;
         long long all;
-        const long long end = tokens_before + block_scan(A, warps, &all);
+        const long long end = tokens_before + block_scan<THREADS>(A, sums[0], &all);
+        const int chunk_begin = (int)min(tokens_before, (long long)max_tokens);
         tokens_before += all;
-        const long long want = (L + (long long)A + page_size - 1) / page_size;
+        const int chunk_end = (int)min(tokens_before, (long long)max_tokens);
+        const int held = pages_of(L, page_size);
+        const long long want = ((long long)L + A + page_size - 1) / page_size;
         const bool fits = i < n && want <= max_pages && end <= max_tokens;
-        const int need = fits ? (int)want - pages_of(L, page_size) : 0;
-        const long long last = pages_before + block_scan(need, warps, &all);
+        const int need = fits ? (int)want - held : 0;
+        const long long last = pages_before + block_scan<THREADS>(need, sums[1], &all);
         pages_before += all;
         const bool served = fits && (need == 0 || last <= F);
-        begin_of[threadIdx.x] = end - A;
-        page_begin[threadIdx.x] = last - need;
+        begin_of[threadIdx.x] = i < n ? (int)min(end - A, (long long)max_tokens) : INT_MAX;
+        page_begin[threadIdx.x] = served ? (int)(last - need) : 0;
         len_of[threadIdx.x] = L;
-        new_of[threadIdx.x] = A;
-        need_of[threadIdx.x] = served ? need : -1;
-        if (i < n) {
+        held_of[threadIdx.x] = served ? held : ~held;
+        if (served && need > 0) atomicMax(&taken, (int)last);
+        sync_all<BLOCKS>();                                   // the arrays are filled, and all blocks have read these lengths
+        if (me == 0 && i < n) {
             lens_out[i] = served ? L + A : L;
-            if (starts) starts[i] = (int)min(end - A, (long long)max_tokens);
+            if (starts) starts[i] = begin_of[threadIdx.x];
         }
-        (void)block_scan(served ? need : 0, warps, &all);
-        taken += all;                    // (its barriers also publish the arrays)
-        for (int r = w; r < min(PG_THREADS, n - base); r += PG_WARPS) {
-            const long long S = begin_of[r];
-            const int Lr = len_of[r], Ar = new_of[r], needed = need_of[r];
-            int *table = tables + (size_t)(base + r) * max_pages;
-            const int have = pages_of(Lr, page_size);
-            for (int k = lane; k < needed; k += 32) table[have + k] = free_pages[F - 1 - (int)(page_begin[r] + k)];
-            __syncwarp();
-            for (int j = lane; j < Ar && S + j < max_tokens; j += 32) {
-                const int at = (int)S + j, pos = (int)min((long long)Lr + j, (long long)INT_MAX);
-                int slot = -1;
-                if (needed >= 0) {
-                    const int page = table[pos / page_size];
-                    if (page >= 0 && page < pages) slot = page * page_size + pos % page_size;
+        for (int t = chunk_begin + me * THREADS + (int)threadIdx.x; t < chunk_end; t += BLOCKS * THREADS) {
+            int r = 0;                                        // the last request that begins at t or before it
+#pragma unroll
+            for (int step = THREADS / 2; step > 0; step >>= 1)
+                if (begin_of[r + step] <= t) r += step;
+            const long long at = (long long)len_of[r] + (t - begin_of[r]);
+            const int pos = (int)min(at, (long long)INT_MAX), held_r = held_of[r];
+            int slot = -1;
+            if (held_r >= 0) {
+                const int k = pos / page_size, off = pos - k * page_size;
+                int *entry = tables + (size_t)(base + r) * max_pages + k;
+                int page;
+                if (k >= held_r) {
+                    page = free_pages[F - 1 - (page_begin[r] + k - held_r)];
+                    if (off == 0) *entry = page;              // (a new page begins with a new token)
+                } else {
+                    page = *entry;
                 }
-                slots[at] = slot;
-                if (positions) positions[at] = pos;
-                if (owners) owners[at] = base + r;
+                if (page >= 0 && page < pages) slot = page * page_size + off;
             }
+            slots[t] = slot;
+            if (positions) positions[t] = pos;
+            if (owners) owners[t] = base + r;
         }
         __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        *free_left = F - (int)taken;
-        if (starts) starts[n] = (int)min(tokens_before, (long long)max_tokens);
-    }
-    for (long long t = tokens_before + threadIdx.x; t < max_tokens; t += PG_THREADS) {
+    for (long long t = tokens_before + me * THREADS + threadIdx.x; t < max_tokens; t += BLOCKS * THREADS) {
         slots[t] = -1;
         if (positions) positions[t] = 0;
         if (owners) owners[t] = -1;
     }
+    sync_all<BLOCKS>();                                       // (all have read free_count, if there was no request)
+    if (me == 0 && threadIdx.x == 0) {
+        *free_left = F - taken;
+        if (starts) starts[n] = (int)min(tokens_before, (long long)max_tokens);
+    }
 }
 
-__global__ void __launch_bounds__(PG_THREADS) release_k(int *free_pages, int *free_out, int *lens_out, const int *free_count, const int *lens,
-                                                        const int *tables, const int *done, int n, int max_pages, int page_size, int pages) {
-    __shared__ long long warps[PG_WARPS];
-    __shared__ long long begin_of[PG_THREADS];
-    __shared__ int held[PG_THREADS], valid[PG_THREADS];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+template <int BLOCKS, int THREADS>
+__global__ void __launch_bounds__(THREADS) release_k(int *free_pages, int *free_out, int *lens_out, const int *free_count, const int *lens,
+                                                     const int *tables, const int *done, int n, int max_pages, int page_size, int pages) {
+    __shared__ long long sums[2][THREADS / 32];
+    __shared__ long long end_of[THREADS];                     // where the entries of the stretch's requests end
+    __shared__ long long found;                               // pages of the pool among this block's entries
+    const int me = BLOCKS == 1 ? 0 : (int)cluster_rank(), lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    let_successor_start();
+    wait_for_predecessor();
     const int F = min(max(*free_count, 0), pages);
     long long before = F;
-    for (int base = 0; base < n; base += PG_THREADS) {
+    for (int base = 0; base < n; base += THREADS) {
         const int i = base + threadIdx.x;
         const bool ends = i < n && done[i] != 0;
         const int L = i < n ? max(lens[i], 0) : 0;
-        held[threadIdx.x] = ends ? min(pages_of(L, page_size), max_pages) : 0;
-        if (i < n) lens_out[i] = ends ? 0 : L;
-        __syncthreads();
-        for (int r = w; r < PG_THREADS; r += PG_WARPS) {
-            const int *table = tables + (size_t)min(base + r, n - 1) * max_pages;
-            int count = 0;
-            for (int k = 0; k < held[r]; k += 32) {
-                const int page = k + lane < held[r] ? table[k + lane] : -1;
-                count += __popc(__ballot_sync(0xffffffffu, page >= 0 && page < pages));
+        long long entries, all;
+        end_of[threadIdx.x] = block_scan<THREADS>(ends ? min(pages_of(L, page_size), max_pages) : 0, sums[0], &entries);
+        sync_all<BLOCKS>();                                   // as in assign_k
+        if (me == 0 && i < n) lens_out[i] = ends ? 0 : L;
+        // a run of entries for each warp, in order; once to count and once to write
+        constexpr int WARPS = BLOCKS * THREADS / 32, AHEAD = 4;
+        const long long each = (entries + WARPS * 32 - 1) / (WARPS * 32) * 32;
+        const long long from = (me * (THREADS / 32) + w) * each, to = min(from + each, entries);
+        auto walk = [&](auto &&use) {
+            int r = 0;
+            if (from < to)
+#pragma unroll
+                for (int step = THREADS / 2; step > 0; step >>= 1)
+                    if (end_of[r + step - 1] <= from) r += step;
+            for (long long f = from + lane; f - lane < to; f += 32 * AHEAD) {
+                int page[AHEAD];
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const long long e = f + 32 * k;
+                    page[k] = -1;
+                    if (e < to) {
+                        while (end_of[r] <= e) ++r;
+                        page[k] = tables[(size_t)(base + r) * max_pages + (e - (r > 0 ? end_of[r - 1] : 0))];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) use(page[k], __ballot_sync(0xffffffffu, page[k] >= 0 && page[k] < pages));
             }
-            if (lane == 0) valid[r] = count;
+        };
+        int mine = 0;
+        walk([&](int, unsigned ok) { mine += __popc(ok); });
+        long long at = block_scan<THREADS>(lane == 31 ? mine : 0, sums[1], &all) - (lane == 31 ? mine : 0);
+        at = before + __shfl_sync(0xffffffffu, at, 31);
+        if (BLOCKS > 1) {
+            if (threadIdx.x == 0) found = all;
+            sync_all<BLOCKS>();
+            all = 0;
+            for (int b = 0; b < BLOCKS; ++b) {
+                const long long x = read_of(&found, b);
+                all += x;
+                if (b < me) at += x;
+            }
         }
-        __syncthreads();
-        long long all;
-        const int mine = valid[threadIdx.x];
-        begin_of[threadIdx.x] = before + block_scan(mine, warps, &all) - mine;
+        walk([&](int page, unsigned ok) {
+            const long long place = at + __popc(ok & ((1u << lane) - 1));
+            if ((ok >> lane & 1) && place < pages) free_pages[place] = page;
+            at += __popc(ok);
+        });
         before += all;
-        __syncthreads();
-        for (int r = w; r < PG_THREADS; r += PG_WARPS) {
-            const int *table = tables + (size_t)min(base + r, n - 1) * max_pages;
-            long long at = begin_of[r];
-            for (int k = 0; k < held[r]; k += 32) {
-                const int page = k + lane < held[r] ? table[k + lane] : -1;
-                const unsigned ok = __ballot_sync(0xffffffffu, page >= 0 && page < pages);
-                const long long to = at + __popc(ok & ((1u << lane) - 1));
-                if ((ok >> lane & 1) && to < pages) free_pages[to] = page;
-                at += __popc(ok);
-            }
-        }
-        __syncthreads();
+        sync_all<BLOCKS>();                                   // (the others have read `found`)
     }
-    if (threadIdx.x == 0) *free_out = (int)min(before, (long long)pages);
+    if (n == 0) sync_all<BLOCKS>();
+    if (me == 0 && threadIdx.x == 0) *free_out = (int)min(before, (long long)pages);
 }
+
+// BLOCKS blocks of one cluster, beside the end of the launch before.
+template <int BLOCKS, typename... P, typename... A>
+int launch_cluster(void (*kernel)(P...), int threads, cudaStream_t st, A... args) {
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = BLOCKS;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = BLOCKS;
+    cfg.blockDim = threads;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = BLOCKS > 1 ? 2 : 1;
+    BMB_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+    count_launch();
+    return BMB_OK;
+}
+
+// Requests and tokens (or table entries) that one block of 256 serves; beyond that, 8 of 1024.
+constexpr int PG_FEW_REQUESTS = 256, PG_FEW = 1024;
 
 int check_pool(const char *what, int n, int max_pages, int page_size, int pages) {
     if (n < 0 || max_pages <= 0 || page_size <= 0 || pages < 0)
@@ -164,8 +252,11 @@ int bmb_pages_assign(int *tables, int *lens_out, int *slots, int *positions, int
     if (max_tokens < 0) return fail(BMB_E_ARG, "pages_assign: max_tokens=%d", max_tokens);
     if (!free_left || !free_count || (pages && !free_pages) || (max_tokens && !slots) || (n && (!tables || !lens_out || !lens || !new_lens)))
         return fail(BMB_E_ARG, "pages_assign: a null pointer");
-    return launch(false, assign_k, 1, PG_THREADS, 0, (cudaStream_t)stream, tables, lens_out, slots, positions, owners, starts, free_left, lens,
-                  new_lens, free_pages, free_count, n, max_pages, page_size, pages, max_tokens);
+    if (n <= PG_FEW_REQUESTS && max_tokens <= PG_FEW)
+        return launch_cluster<1>(assign_k<1, 256>, 256, (cudaStream_t)stream, tables, lens_out, slots, positions, owners, starts, free_left, lens,
+                                 new_lens, free_pages, free_count, n, max_pages, page_size, pages, max_tokens);
+    return launch_cluster<PG_CLUSTER>(assign_k<PG_CLUSTER, PG_MOST>, PG_MOST, (cudaStream_t)stream, tables, lens_out, slots, positions, owners, starts,
+                                      free_left, lens, new_lens, free_pages, free_count, n, max_pages, page_size, pages, max_tokens);
 }
 
 int bmb_pages_release(int *free_pages, int *free_out, int *lens_out, const int *free_count, const int *lens, const int *tables, const int *done,
@@ -173,8 +264,11 @@ int bmb_pages_release(int *free_pages, int *free_out, int *lens_out, const int *
     BMB_TRY(check_pool("pages_release", n, max_pages, page_size, pages));
     if (!free_out || !free_count || (pages && !free_pages) || (n && (!tables || !lens_out || !lens || !done)))
         return fail(BMB_E_ARG, "pages_release: a null pointer");
-    return launch(false, release_k, 1, PG_THREADS, 0, (cudaStream_t)stream, free_pages, free_out, lens_out, free_count, lens, tables, done, n,
-                  max_pages, page_size, pages);
+    if (n <= PG_FEW_REQUESTS && (long long)n * max_pages <= PG_FEW)
+        return launch_cluster<1>(release_k<1, 256>, 256, (cudaStream_t)stream, free_pages, free_out, lens_out, free_count, lens, tables, done, n,
+                                 max_pages, page_size, pages);
+    return launch_cluster<PG_CLUSTER>(release_k<PG_CLUSTER, PG_MOST>, PG_MOST, (cudaStream_t)stream, free_pages, free_out, lens_out, free_count, lens,
+                                      tables, done, n, max_pages, page_size, pages);
 }
 
 }  // extern "C"
