@@ -63,6 +63,10 @@ class KvCache(C.Structure):
         return c
 
 
+class BatchSampling(C.Structure):
+    _fields_ = [(n, _f) for n in ("temperature", "repetition", "frequency", "presence")] + [("stop_token", _i), ("cache_type", _i)]
+
+
 class LogitRules(C.Structure):
     _fields_ = [(n, _p) for n in ("history", "history_lens", "prompt_lens", "repetition", "frequency", "presence", "bias_ids", "bias",
                                   "bias_lens", "allowed")] + [(n, _i) for n in ("history_stride", "bias_stride", "allowed_stride")]
@@ -184,6 +188,7 @@ SIGNATURES = {
     "bmb_trainer_load": (_i, [_p, C.c_char_p, _i, C.POINTER(_i)]),
     "bmb_trainer_next_token_probs": (_i, [_p, _p, _i, _p]),
     "bmb_trainer_generate": (_i, [_p, _i, _i, _u, _f, _p]),
+    "bmb_trainer_generate_batch": (_i, [_p, _i, _p, _i, _p, _i, _u, C.POINTER(BatchSampling), _p]),
     "bmb_trainer_stream": (_p, [_p]),
     "bmb_trainer_profile": (_i, [_p, _i]),
     "bmb_trainer_profile_read": (_i, [_p, C.POINTER(_d), C.POINTER(_d), C.POINTER(_ll), C.POINTER(_ll)]),
@@ -229,10 +234,14 @@ def ptr(t):
 _PLAIN = frozenset((int, float, type(None), KvCache, LogitRules))      # what ctypes takes as it is
 
 
+def _arg(a):
+    address = getattr(a, "data_ptr", None)
+    return address() if address is not None else ptr(a) if hasattr(a, "ctypes") else a
+
+
 def call(name, *args):
     """Call a status-returning entry point with tensors turned into pointers."""
-    conv = [a if a.__class__ in _PLAIN or not (hasattr(a, "data_ptr") or hasattr(a, "ctypes")) else ptr(a) for a in args]
-    status = getattr(_lib or lib(), name)(*conv)
+    status = getattr(_lib or lib(), name)(*[a if a.__class__ in _PLAIN else _arg(a) for a in args])
     if status:
         check(status, name)
 
@@ -339,6 +348,17 @@ class Trainer:
         out = (C.c_int * max(steps, 1))()
         check(lib().bmb_trainer_generate(self.h, start_token, steps, seed, temperature, out), "bmb_trainer_generate")
         return list(out[:steps])
+
+    def generate_batch(self, prompts, steps, seed, temperature=1.0, repetition=1.0, frequency=0.0, presence=0.0, stop=-1, cache=TYPE_FP32):
+        """The tokens drawn behind each of the prompts (lists of tokens), up to and with the stop token."""
+        n, width = len(prompts), max([len(p) for p in prompts] + [1])
+        flat = (C.c_int * max(n * width, 1))()
+        for i, p in enumerate(prompts):
+            flat[i * width:i * width + len(p)] = list(p)
+        lens, out = (C.c_int * max(n, 1))(*[len(p) for p in prompts]), (C.c_int * max(n * steps, 1))()
+        how = BatchSampling(temperature, repetition, frequency, presence, stop, cache)
+        check(lib().bmb_trainer_generate_batch(self.h, n, flat, width, lens, steps, seed, C.byref(how), out), "bmb_trainer_generate_batch")
+        return [[t for t in out[i * steps:(i + 1) * steps] if t >= 0] for i in range(n)]
 
     def close(self):
         if self.h:

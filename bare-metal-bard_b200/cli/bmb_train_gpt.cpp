@@ -37,6 +37,8 @@ struct Options {
     float temperature = 0.8f;
     unsigned seed = 1337;
     bool use_flash = true, alloc_only = false, synthetic = false, save_optimizer = false;
+    int texts = 1;                       // drawn at once; with more than one, or with penalties, each within the context
+    float repetition = 1.0f, frequency = 0.0f, presence = 0.0f;
     int synthetic_vocab = 50304, math = BMB_MATH_FP32, fused = -1;
 };
 
@@ -131,10 +133,24 @@ struct Run {
         int start = 0;
         for (size_t i = 0; i < corpus.itos.size(); ++i)
             if (corpus.itos[i] == '\n') { start = (int)i; break; }
-        std::vector<int> toks((size_t)std::max(len, 1));
-        CHECK(bmb_trainer_generate(t, start, len, seed, o.temperature, toks.data()));
+        const bool together = o.texts > 1 || o.repetition != 1.0f || o.frequency != 0.0f || o.presence != 0.0f;
+        if (together) len = std::min(len, o.T - 1);
+        std::vector<int> toks((size_t)std::max(len, 1) * o.texts);
+        if (together) {
+            const std::vector<int> starts(o.texts, start), ones(o.texts, 1);
+            const bmb_batch_sampling how{o.temperature, o.repetition, o.frequency, o.presence, -1, BMB_TYPE_FP32};
+            CHECK(bmb_trainer_generate_batch(t, o.texts, starts.data(), 1, ones.data(), len, seed, &how, toks.data()));
+        } else {
+            CHECK(bmb_trainer_generate(t, start, len, seed, o.temperature, toks.data()));
+        }
         std::string s;
-        for (int i = 0; i < len; ++i) s.push_back((size_t)toks[i] < corpus.itos.size() ? corpus.itos[toks[i]] : '?');
+        for (int j = 0; j < o.texts; ++j) {
+            if (j > 0) s += "\n  [text " + std::to_string(j + 1) + "] ------------------------------------------\n";
+            for (int i = 0; i < len; ++i) {
+                const int tok = toks[(size_t)j * len + i];
+                s.push_back((size_t)tok < corpus.itos.size() ? corpus.itos[tok] : '?');
+            }
+        }
         return s;
     }
 };
@@ -182,6 +198,10 @@ int main(int argc, char **argv) {
         else if (!strcmp(a, "--resume")) o.resume_path = val();
         else if (!strcmp(a, "--len")) o.sample_len = atoi(val());
         else if (!strcmp(a, "--temp")) o.temperature = (float)atof(val());
+        else if (!strcmp(a, "--texts")) o.texts = std::max(atoi(val()), 1);
+        else if (!strcmp(a, "--repetition")) o.repetition = (float)atof(val());
+        else if (!strcmp(a, "--frequency")) o.frequency = (float)atof(val());
+        else if (!strcmp(a, "--presence")) o.presence = (float)atof(val());
         else if (!strcmp(a, "--alloc-only")) o.alloc_only = true;
         else if (!strcmp(a, "--unfused")) o.use_flash = false;
         else if (!strcmp(a, "--synthetic")) o.synthetic = true;

@@ -168,6 +168,18 @@ struct DecodeModel {
     float scale;
 };
 size_t decode_exchange(int C);
+// A model as generate_texts reads it: weights of products as wflag says they are (W), the others as stored.
+struct ServeModel {
+    const float *wte, *wpe, *wte_w, *ln1w, *ln1b, *qkvw, *qkvb, *apw, *apb, *ln2w, *ln2b, *fcw, *fcb, *fpw, *fpb, *lnfw, *lnfb;
+    int math, wflag, attention;   // attention: the configuration for prompts
+    int C, NH, L, V, Vp;
+    cudaStream_t st;              // the thread's current one
+};
+int generate_texts(const ServeModel &m, int n, const int *host_prompts, int prompt_stride, const int *host_prompt_lens, int steps, unsigned seed,
+                   const bmb_batch_sampling &how, int *host_tokens_out);
+// The draw of src/train_gpt.cu:79-95: probabilities (overwritten where temperature is not 1) to the power 1 / temperature, and the first token whose
+// cumulative one is above coin.
+int draw_token(float *probs, int V, float temperature, float coin);
 // The position's row before layer `first` (which may be L: the head alone) is x0, or x0 + x1 where that is given. `launch` counts the launches with one
 // exchange: another one each time.
 int decode_position(const DecodeModel &m, const float *x0, const float *x1, int first, int pos, unsigned launch, cudaStream_t st);

@@ -83,6 +83,15 @@ int run_write(const bmb_kv_cache &c, const float *k, const float *v, long long r
 constexpr int PA_WARPS = 4, PA_THREADS = 32 * PA_WARPS, PA_STAGES = 3, PA_TILE = 4096, PA_ROWS = 8;
 constexpr int PA_BLOCKS = 2;            // blocks an SM
 constexpr int PA_MOST_BLOCKS = 512;
+// Where heads are no more than blocks and short, a block takes each head alone, a quarter of its tiles a warp: no line to find a place in
+// and no second launch, which together are 3 to 4 us; but a warp then has up to tiles / 4 of them in a row, 0.6 us each, where the line spreads
+// all over the GPU.  Measured, alone / line, at the longest length the tables hold: 6 heads of 64 fp32 of 8, 16 and 24 tiles 5.7 / 7.6,
+// 8.2 / 7.7, 10.5 / 7.8 us; 96 heads bf16 of 16 and 24 tiles 9.9 / 10.9, 13.0 / 11.7; 256 heads of 128 fp16 of 32 tiles 16.0 / 25.0.  Above
+// PA_ALONE_TILES one long request among short ones would cost too much.
+constexpr int PA_ALONE_TILES = 32;
+inline bool heads_alone(long long heads, int tiles, int blocks) {
+    return heads <= blocks && tiles <= PA_ALONE_TILES && tiles * (blocks - heads) <= 16LL * blocks;
+}
 constexpr size_t PA_SMEM = 112 * 1024;   // dynamic shared memory with which two blocks fit an SM
 
 // All places in a line: requests in order, of each its (virtual) heads, of each its tiles and one place more, without work of its own, for
@@ -201,6 +210,7 @@ struct Attend {
     int max_pages;
     float scale;
     bool staged, aligned_q;      // queries are staged in shared memory, 16 bytes at a time
+    bool alone;                  // a block for each head, not the line
     Shape s;
     Parts w;
 };
@@ -216,7 +226,10 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
     __shared__ long long warp_total[PA_WARPS];                                   // (at the start)
     __shared__ float part_m[PA_WARPS][2][PA_ROWS], part_l[PA_WARPS][2][PA_ROWS];
     __shared__ int4 part_of[PA_WARPS][2];                                        // request, virtual head, 1 begins + 2 ends there, 1 (0: none)
-    __shared__ float weight[2 * PA_WARPS][PA_ROWS];
+    __shared__ __align__(16) float weight[2 * PA_WARPS][PA_ROWS];                // (and at the start:)
+    struct RunBegin { long long in; int request; };                              // `in` places behind the first one of this request
+    RunBegin *run_begin = reinterpret_cast<RunBegin *>(weight);
+    static_assert(sizeof(weight) >= PA_WARPS * sizeof(RunBegin), "");
     __shared__ int last_block[PA_WARPS + 1];                                      // that has a part of the head a warp has begun and not ended
     int *group_of = reinterpret_cast<int *>(warp_total), &groups = last_block[PA_WARPS];      // first entry, last one << 8, what they say together << 16
     static_assert(sizeof(warp_total) >= 2 * PA_WARPS * sizeof(int), "");
@@ -225,47 +238,61 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rows_kept = min(s.group, PA_ROWS);
     unsigned char *ring = smem + w * (PA_STAGES * 2 * PA_TILE);
-    // (of the dynamic memory: the rings, a part of a head for each warp, and before the first load how many places (of one head each) lie before each stretch)
-    long long *before = reinterpret_cast<long long *>(smem);
+    // (dynamic memory: the rings, a part of a head for each warp, staged queries)
     float *first_part = reinterpret_cast<float *>(smem + PA_WARPS * PA_STAGES * 2 * PA_TILE) + w * rows_kept * HS;   // [rows][HS]
     let_successor_start();
     wait_for_predecessor();
 
-    // ---- how many places (of one head each) lie before each thread's stretch of requests ----
-    const int stretch = s.stretch();
-    long long mine = 0;
     const int len_here = (int)blockIdx.x < s.n ? p.lens[blockIdx.x] : 1;
-    for (int i = 0, r = threadIdx.x * stretch; i < stretch && r < s.n; ++i, ++r) mine += s.places(p.lens[r]);
-    long long sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += u;
-    }
-    if (lane == 31) warp_total[w] = sum;
     if (lane < 2) part_of[w][lane] = make_int4(0, 0, 0, 0);
-    __syncthreads();
-    long long total = 0;
-    for (int i = 0; i < PA_WARPS; ++i) {
-        if (i < w) sum += warp_total[i];
-        total += warp_total[i];
+    Place here;
+    Line line(0, 1);
+    long long begin = 0;                                      // of this warp's run in the line, and its places, from 0: the next one and the end
+    int at_place = 0, end = 0;
+    if (p.alone) {
+        here.request = blockIdx.x / s.vheads;
+        here.vhead = blockIdx.x - here.request * s.vheads;
+        here.len = s.length(p.lens[here.request]);
+        here.tiles = s.tiles(here.len);
+        here.tile = (int)((long long)here.tiles * w / PA_WARPS);
+        end = (int)((long long)here.tiles * (w + 1) / PA_WARPS) - here.tile;
+        __syncthreads();
+    } else {
+        // how many places (of one head each) lie before each thread's stretch of requests
+        const int stretch = s.stretch();
+        long long mine = 0;
+        for (int i = 0, r = threadIdx.x * stretch; i < stretch && r < s.n; ++i, ++r) mine += s.places(p.lens[r]);
+        long long sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += u;
+        }
+        if (lane == 31) warp_total[w] = sum;
+        __syncthreads();
+        long long total = 0;
+        for (int i = 0; i < PA_WARPS; ++i) {
+            if (i < w) sum += warp_total[i];
+            total += warp_total[i];
+        }
+        line = Line(total * s.vheads, gridDim.x * PA_WARPS);
+        // the stretch that a run's first place lies in says so
+        if (mine > 0)
+#pragma unroll
+            for (int i = 0; i < PA_WARPS; ++i) {
+                const long long in = line.begin(blockIdx.x * PA_WARPS + i) - (sum - mine) * s.vheads;
+                if (in >= 0 && in < mine * s.vheads) run_begin[i] = {in, (int)threadIdx.x * stretch};
+            }
+        __syncthreads();
+        const int run = blockIdx.x * PA_WARPS + w;
+        if (total > 0 && run < line.warps) {
+            begin = line.begin(run);
+            end = (int)(line.begin(run + 1) - begin);
+            at_place = here.set(s, p.lens, run_begin[w].request, run_begin[w].in);
+        }
     }
-    before[threadIdx.x] = sum - mine;
-    __syncthreads();
 
-    const Line line(total * s.vheads, gridDim.x * PA_WARPS);
-    const int run = blockIdx.x * PA_WARPS + w;
-    // the stretch that holds the run's first place: the last one with no more places before it
-    int at = 0;
-    for (int i = lane; i < PA_THREADS; i += 32)
-        at += __popc(__ballot_sync(0xffffffffu, before[i] * s.vheads <= line.begin(run) && (long long)i * stretch < s.n));
-    const long long before_run = before[at > 0 ? at - 1 : 0] * s.vheads;
-    __syncthreads();
-    if (total > 0 && run < line.warps) {
-        const long long begin = line.begin(run);
-        const int end = (int)(line.begin(run + 1) - begin);   // places of the run, from 0
-        Place here;
-        int at_place = here.set(s, p.lens, (at - 1) * stretch, begin - before_run);
+    if (at_place < end) {
         Place load = here;                                    // the tile that is loaded next
         int load_place = at_place;
         // queries of the first row of a head
@@ -425,7 +452,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
         };
 
         int next_page[HELD];                                  // for the tile that is loaded next
-        if (at_place < end) {
+        {
             float x[HS / 4];
             read_queries(queries(here), x);
             heads_read ^= here.tile == 0;                     // (its first tile brings them again)
@@ -637,7 +664,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
         if (first) group_of[__popc(firsts & ((1u << lane) - 1))] = lane | last << 8 | flags << 16;
         if (first && flags == 1) p.w.begun[blockIdx.x] = make_int4(of.x, of.y, last_block[lane >> 1], 1);
         if (lane == 0) groups = __popc(firsts);
-        if (!__any_sync(0xffffffffu, first && flags == 1) && lane == 0) p.w.begun[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (!__any_sync(0xffffffffu, first && flags == 1) && lane == 0 && !p.alone) p.w.begun[blockIdx.x] = make_int4(0, 0, 0, 0);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < groups * rows_kept * (HS / 4); i += PA_THREADS) {
@@ -694,6 +721,7 @@ __global__ void __launch_bounds__(PJ_THREADS) attend_join_k(const __grid_constan
     __shared__ float by[PA_MOST_BLOCKS], red[32], sum[ACROSS][HS];
     const Shape s = p.s;
     const int r = blockIdx.y, d = threadIdx.x % (HS / 4) * 4, a = threadIdx.x / (HS / 4);
+    let_successor_start();
     wait_for_predecessor();
     const int4 of = p.w.begun[blockIdx.x];
     if (!of.w || r >= min(PA_ROWS, s.group - (of.y % s.parts) * PA_ROWS)) return;
@@ -707,6 +735,14 @@ __global__ void __launch_bounds__(PJ_THREADS) attend_join_k(const __grid_constan
         l[k] = i < n ? p.w.l[row(i)] : 0.0f;
         top = fmaxf(top, m[k]);
     }
+    constexpr int AHEAD = 4;
+    float4 v[AHEAD];
+    auto read = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            v[k] = i + k * ACROSS < n ? *reinterpret_cast<const float4 *>(p.w.o + row(i + k * ACROSS) * HS + d) : make_float4(0, 0, 0, 0);
+    };
+    read(a);
     // (a maximum of -inf, which block_reduce raises to the lowest number, has no weights: l is 0 throughout, or NaN)
     top = block_reduce<true>(top, red);
 #pragma unroll
@@ -717,18 +753,16 @@ __global__ void __launch_bounds__(PJ_THREADS) attend_join_k(const __grid_constan
     }
     all = block_reduce<false>(all, red);                      // (its barriers also publish the weights)
     float x[4] = {};
-    for (int i = a; i < n; i += 4 * ACROSS) {
-        float4 v[4];
+    for (int i = a; i < n; i += AHEAD * ACROSS) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = i + k * ACROSS < n ? *reinterpret_cast<const float4 *>(p.w.o + row(i + k * ACROSS) * HS + d) : make_float4(0, 0, 0, 0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < AHEAD; ++k) {
             const float w = i + k * ACROSS < n ? by[i + k * ACROSS] : 0.0f;
             x[0] = fmaf(v[k].x, w, x[0]);
             x[1] = fmaf(v[k].y, w, x[1]);
             x[2] = fmaf(v[k].z, w, x[2]);
             x[3] = fmaf(v[k].w, w, x[3]);
         }
+        read(i + AHEAD * ACROSS);
     }
     *reinterpret_cast<float4 *>(&sum[a][d]) = make_float4(x[0], x[1], x[2], x[3]);
     __syncthreads();
@@ -788,7 +822,8 @@ int run_attend(Attend &p, cudaStream_t st) {
         BMB_CUDA(cudaFuncSetAttribute(attend_k<T, HS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PA_SMEM));
         prepared.fetch_or(bit, std::memory_order_relaxed);
     }
-    BMB_TRY(launch_in_chain(attend_k<T, HS>, blocks, PA_THREADS, least + (p.staged ? PA_WARPS * 2 * part : 0), st, p));
+    BMB_TRY(launch_in_chain(attend_k<T, HS>, p.alone ? p.s.n * p.s.vheads : blocks, PA_THREADS, least + (p.staged ? PA_WARPS * 2 * part : 0), st, p));
+    if (p.alone) return BMB_OK;
     return launch_in_chain(attend_join_k<HS>, dim3(blocks, rows), PJ_THREADS, 0, st, p);
 }
 template <typename T>
@@ -908,6 +943,7 @@ int bmb_paged_attention(float *out, float *lse, const float *q, const bmb_kv_cac
     p.s = attend_shape(n, heads, cache->heads, hs, cache->type, max_pages * cache->page_size);
     if ((double)n * p.s.vheads * p.s.places(p.s.cap) > 1e12)
         return fail(BMB_E_LIMIT, "paged_attention: %d requests of %d tokens", n, p.s.cap);
+    p.alone = heads_alone((long long)n * p.s.vheads, p.s.tiles(p.s.cap), blocks);
     p.w.o = (float *)workspace;
     p.w.m = p.w.o + (size_t)blocks * 2 * PA_ROWS * hs;
     p.w.l = p.w.m + (size_t)blocks * 2 * PA_ROWS;

@@ -10,6 +10,7 @@
 #include "common.cuh"
 #include <cmath>
 #include <cstring>
+#include <exception>
 #include <random>
 #include <string>
 #include <vector>
@@ -1355,15 +1356,7 @@ int bmb_trainer_generate(bmb_trainer *t, int start_token, int steps, unsigned se
         } else {
             BMB_TRY(bmb_trainer_next_token_probs(t, ctx.data(), cur_len - 1, row.data()));
         }
-        if (temperature != 1.0f) {
-            float sum = 0.0f;
-            for (int i = 0; i < V; ++i) { row[i] = powf(row[i], 1.0f / temperature); sum += row[i]; }
-            for (int i = 0; i < V; ++i) row[i] /= sum;
-        }
-        const float coin = uni(rng);
-        float cdf = 0.0f;
-        int tok = V - 1;
-        for (int i = 0; i < V; ++i) { cdf += row[i]; if (coin < cdf) { tok = i; break; } }
+        const int tok = draw_token(row.data(), V, temperature, uni(rng));
         host_tokens_out[s] = tok;
         if (cur_len < T) ctx[cur_len++] = tok;
         else {                               // context full: slide the window left by one
@@ -1372,6 +1365,40 @@ int bmb_trainer_generate(bmb_trainer *t, int start_token, int steps, unsigned se
         }
     }
     return BMB_OK;
+}
+
+int bmb_trainer_generate_batch(bmb_trainer *t, int n, const int *host_prompts, int prompt_stride, const int *host_prompt_lens, int steps, unsigned seed,
+                               const bmb_batch_sampling *how, int *host_tokens_out) {
+    if (!t || n < 0 || steps < 0 || !how || !(how->temperature > 0.0f) || !(how->repetition > 0.0f) || how->frequency != how->frequency ||
+        how->presence != how->presence || how->cache_type < BMB_TYPE_FP32 || how->cache_type > BMB_TYPE_FP16)
+        return fail(BMB_E_ARG, "trainer_generate_batch: bad argument");
+    if (n == 0 || steps == 0) return BMB_OK;
+    if (!host_prompts || !host_prompt_lens || !host_tokens_out) return fail(BMB_E_ARG, "trainer_generate_batch: a null pointer");
+    const bmb_train_config &c = t->c;
+    const int hs = c.n_embd / c.n_head;
+    if (hs != 32 && hs != 64 && hs != 128) return fail(BMB_E_UNSUPPORTED, "trainer_generate_batch: head size %d (32, 64 and 128 are served)", hs);
+    for (int i = 0; i < n; ++i) {
+        const int len = host_prompt_lens[i];
+        if (len < 1 || len > prompt_stride) return fail(BMB_E_ARG, "trainer_generate_batch: a prompt of %d tokens in rows of %d", len, prompt_stride);
+        if ((long long)len + steps > c.max_seq_len)
+            return fail(BMB_E_LIMIT, "trainer_generate_batch: %d tokens and %d more are beyond the model's %d positions", len, steps, c.max_seq_len);
+        for (int j = 0; j < len; ++j) {
+            const int token = host_prompts[(size_t)i * prompt_stride + j];
+            if (token < 0 || token >= c.vocab_size) return fail(BMB_E_ARG, "trainer_generate_batch: token %d of prompt %d is %d", j, i, token);
+        }
+    }
+    Scope sc(t);
+    const Dims d = dims_of(t);
+    const auto P = [&](int tensor) { return d.P + t->poff[tensor]; };
+    const auto W = [&](int tensor) { return d.W + t->poff[tensor]; };
+    const ServeModel m{P(P_WTE), P(P_WPE), W(P_WTE), P(P_LN1W), P(P_LN1B), W(P_QKVW), P(P_QKVB), W(P_APW), P(P_APB), P(P_LN2W), P(P_LN2B), W(P_FCW), P(P_FCB),
+                       W(P_FPW), P(P_FPB), P(P_LNFW), P(P_LNFB), c.math, d.wflag & BMB_GEMM_B_ROUNDED, attn_cfg(c), d.C, d.NH, d.L, d.V, d.Vp, t->st};
+    try {
+        BMB_TRY(generate_texts(m, n, host_prompts, prompt_stride, host_prompt_lens, steps, seed, *how, host_tokens_out));
+    } catch (const std::exception &e) {
+        return fail(BMB_E_LIMIT, "trainer_generate_batch: %s", e.what());
+    }
+    return check_kernel_status();
 }
 
 }  // extern "C"

@@ -507,6 +507,19 @@ int bmb_trainer_next_token_probs(bmb_trainer *t, const int *host_tokens, int pos
  * the window sliding once the context is full.  host_tokens_out receives the drawn token ids. Blocks. */
 int bmb_trainer_generate(bmb_trainer *t, int start_token, int steps, unsigned seed, float temperature,
                          int *host_tokens_out);
+/* Several texts at once: text i begins with the host_prompt_lens[i] (at least 1) tokens of row i of host_prompts ([n][prompt_stride]) and draws
+ * `steps` tokens as bmb_trainer_generate does, with mt19937(seed + i), from logits that the penalties have gone over (bmb_logits_adjust over
+ * its prompt and what it drew; 1, 0, 0: none).  A text that draws stop_token ends with it (-1: none does).  host_tokens_out ([n][steps]) receives
+ * the draws, -1 behind a text's end.  Prompts go through the model in one pass, then a row for each text and step, with keys and values
+ * of cache_type in pages (bmb_pages_assign to bmb_pages_release above).  Each prompt and its draws fit the model's positions
+ * (BMB_E_LIMIT): there is no sliding window.  Head sizes 32, 64 and 128.  Blocks; memory is taken for the call and given back.  Probabilities
+ * are bmb_trainer_generate's up to rounding (of cache_type's, for keys and values). */
+typedef struct bmb_batch_sampling {
+    float temperature, repetition, frequency, presence;
+    int stop_token, cache_type;
+} bmb_batch_sampling;
+int bmb_trainer_generate_batch(bmb_trainer *t, int n, const int *host_prompts, int prompt_stride, const int *host_prompt_lens, int steps,
+                               unsigned seed, const bmb_batch_sampling *how, int *host_tokens_out);
 /* The CUDA stream every step of this trainer is enqueued on (for events). */
 void *bmb_trainer_stream(bmb_trainer *t);
 /* Per-call event timing of the GEMMs inside steps (on = 1 / off = 0); the
