@@ -4,15 +4,17 @@
 // Both are sums over requests in their order (where a request's tokens and pages begin) and stores that follow from them.  What they
 // move is little, so what they take is the chain of loads: lengths, then pages.  A block counts a stretch of requests with a thread
 // each, and tokens (of assign) or table entries (of release) are then dealt to threads whatever requests they are of.  Few
-// of them: one block.  Many: a cluster of 8, each of which counts all of them, with the block number of tokens or entries divided over the
-// cluster; lengths are read by all before any is overwritten, which a cluster's barrier can say and a grid cannot.
+// of them: one block.  Many: a cluster of 8, each of which counts all requests and takes an eighth of the tokens or entries; lengths are
+// read by all before any is overwritten, which a cluster's barrier can say and a grid cannot.
 #include "common.cuh"
 #include <climits>
+#include <type_traits>
 
 namespace bmb {
 namespace {
 
 constexpr int PG_CLUSTER = 8, PG_MOST = 1024;
+template <int V> using Int = std::integral_constant<int, V>;
 
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
@@ -227,8 +229,11 @@ int launch_cluster(void (*kernel)(P...), int threads, cudaStream_t st, A... args
     return BMB_OK;
 }
 
-// Requests and tokens (or table entries) that one block of 256 serves; beyond that, 8 of 1024.
-constexpr int PG_FEW_REQUESTS = 256, PG_FEW = 1024;
+// Up to 256 requests and 1024 tokens (or table entries, by the tables' size): one block of 256 threads.  Up to 2048 tokens or 8192 entries: one of
+// 1024.  Beyond: a cluster of 8.  Measured, us: 64 tokens 3.0 with 256 threads, 3.9 with 1024; 1424 tokens of 256 requests 5.9, 5.0 and
+// 5.3 with the cluster; 15 thousand tokens 15.7 with 1024, 6.0 with the cluster.  Release, tables of 1024 entries 4.2 and 4.2; of 4000
+// 7.3, 5.3 and 7.2; of 62 thousand 13.5 with 1024 and 7.9 with the cluster.
+constexpr int PG_FEW_REQUESTS = 256, PG_FEW = 1024, PG_SOME_TOKENS = 2048, PG_SOME_ENTRIES = 8192;
 
 int check_pool(const char *what, int n, int max_pages, int page_size, int pages) {
     if (n < 0 || max_pages <= 0 || page_size <= 0 || pages < 0)
@@ -252,11 +257,13 @@ int bmb_pages_assign(int *tables, int *lens_out, int *slots, int *positions, int
     if (max_tokens < 0) return fail(BMB_E_ARG, "pages_assign: max_tokens=%d", max_tokens);
     if (!free_left || !free_count || (pages && !free_pages) || (max_tokens && !slots) || (n && (!tables || !lens_out || !lens || !new_lens)))
         return fail(BMB_E_ARG, "pages_assign: a null pointer");
-    if (n <= PG_FEW_REQUESTS && max_tokens <= PG_FEW)
-        return launch_cluster<1>(assign_k<1, 256>, 256, (cudaStream_t)stream, tables, lens_out, slots, positions, owners, starts, free_left, lens,
-                                 new_lens, free_pages, free_count, n, max_pages, page_size, pages, max_tokens);
-    return launch_cluster<PG_CLUSTER>(assign_k<PG_CLUSTER, PG_MOST>, PG_MOST, (cudaStream_t)stream, tables, lens_out, slots, positions, owners, starts,
-                                      free_left, lens, new_lens, free_pages, free_count, n, max_pages, page_size, pages, max_tokens);
+    auto run = [&](auto blocks, auto threads) {
+        constexpr int B = decltype(blocks)::value, N = decltype(threads)::value;
+        return launch_cluster<B>(assign_k<B, N>, N, (cudaStream_t)stream, tables, lens_out, slots, positions, owners, starts, free_left, lens, new_lens,
+                                 free_pages, free_count, n, max_pages, page_size, pages, max_tokens);
+    };
+    if (n <= PG_FEW_REQUESTS && max_tokens <= PG_FEW) return run(Int<1>(), Int<256>());
+    return max_tokens <= PG_SOME_TOKENS ? run(Int<1>(), Int<PG_MOST>()) : run(Int<PG_CLUSTER>(), Int<PG_MOST>());
 }
 
 int bmb_pages_release(int *free_pages, int *free_out, int *lens_out, const int *free_count, const int *lens, const int *tables, const int *done,
@@ -264,11 +271,14 @@ int bmb_pages_release(int *free_pages, int *free_out, int *lens_out, const int *
     BMB_TRY(check_pool("pages_release", n, max_pages, page_size, pages));
     if (!free_out || !free_count || (pages && !free_pages) || (n && (!tables || !lens_out || !lens || !done)))
         return fail(BMB_E_ARG, "pages_release: a null pointer");
-    if (n <= PG_FEW_REQUESTS && (long long)n * max_pages <= PG_FEW)
-        return launch_cluster<1>(release_k<1, 256>, 256, (cudaStream_t)stream, free_pages, free_out, lens_out, free_count, lens, tables, done, n,
-                                 max_pages, page_size, pages);
-    return launch_cluster<PG_CLUSTER>(release_k<PG_CLUSTER, PG_MOST>, PG_MOST, (cudaStream_t)stream, free_pages, free_out, lens_out, free_count, lens,
-                                      tables, done, n, max_pages, page_size, pages);
+    auto run = [&](auto blocks, auto threads) {
+        constexpr int B = decltype(blocks)::value, N = decltype(threads)::value;
+        return launch_cluster<B>(release_k<B, N>, N, (cudaStream_t)stream, free_pages, free_out, lens_out, free_count, lens, tables, done, n, max_pages,
+                                 page_size, pages);
+    };
+    const long long entries = (long long)n * max_pages;
+    if (n <= PG_FEW_REQUESTS && entries <= PG_FEW) return run(Int<1>(), Int<256>());
+    return entries <= PG_SOME_ENTRIES ? run(Int<1>(), Int<PG_MOST>()) : run(Int<PG_CLUSTER>(), Int<PG_MOST>());
 }
 
 }  // extern "C"
