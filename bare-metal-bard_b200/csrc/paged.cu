@@ -163,6 +163,12 @@ __device__ __forceinline__ void mma8(float (&c)[4], const float (&a)[4], float b
                  : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])), "r"(__float_as_uint(a[3])),
                    "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
+// 2^x by the special-function unit, results below 2^-126 as 0 (exp2f's steps to keep those are 3 instructions more).
+__device__ __forceinline__ float two_to(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 template <bool TRANS>
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     if (TRANS)
@@ -192,6 +198,18 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&out)[pieces])
     }
 }
 
+// n / d for 0 <= n < 2^31 and one d: the high half of n times ceil(2^(32 + bits) / d) - 2^32, bits such that 2^bits >= d.  (The division
+// of unknown numbers takes 20 instructions.)
+struct Divide {
+    unsigned by, mul, bits;
+    Divide() = default;
+    explicit Divide(unsigned d) : by(d), bits(0) {
+        while (bits < 31 && (1u << bits) < d) ++bits;
+        mul = (unsigned)(((1ULL << 32) * ((1ULL << bits) - d)) / d + 1);
+    }
+    __device__ __forceinline__ unsigned quotient(unsigned n) const { return (unsigned)(((unsigned long long)__umulhi(n, mul) + n) >> bits); }
+};
+
 // Rows of a head in the workspace: of a block, the part of the head that it ends (0) and of the one that it begins (1).
 struct Parts {
     float *o, *m, *l;      // [blocks][2][PA_ROWS][HS], [blocks][2][PA_ROWS]
@@ -208,6 +226,7 @@ struct Attend {
     const int *tables, *lens;
     long long q_stride, out_stride;
     int max_pages;
+    Divide page_size;
     float scale;
     bool staged, aligned_q;      // queries are staged in shared memory, 16 bytes at a time
     bool alone;                  // a block for each head, not the line
@@ -301,39 +320,46 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
         };
         // ---- the ring ----
         constexpr int HELD = (KEYS + 31) / 32;
-        // pages of the rows that this lane looks up
-        auto look_up = [&](const Place &x, int (&page)[HELD]) {
+        // pages of the rows that this lane looks up, and their places in them
+        struct Rows { int page[HELD], in_page[HELD]; };
+        auto look_up = [&](const Place &x, Rows &rows) {
+            const int *table = p.tables + (size_t)x.request * p.max_pages;
 #pragma unroll
             for (int i = 0; i < HELD; ++i) {
-                const unsigned key = (unsigned)x.tile * KEYS + i * 32 + lane;
-                page[i] = (KEYS >= 32 || lane < KEYS) && key < (unsigned)x.len ? p.tables[(size_t)x.request * p.max_pages + key / (unsigned)p.c.page_size] : -1;
+                const unsigned key = (unsigned)x.tile * KEYS + i * 32 + lane, k = p.page_size.quotient(key);
+                rows.in_page[i] = (int)(key - k * p.page_size.by);
+                rows.page[i] = (KEYS >= 32 || lane < KEYS) && key < (unsigned)x.len ? table[k] : -1;
             }
         };
         unsigned valid[PA_STAGES][HELD];                      // rows that count, of each slot
         int heads_loaded = 0, heads_read = 0;                 // the staging buffer that is next (of two)
         float *staged_q = reinterpret_cast<float *>(smem + PA_WARPS * (PA_STAGES * 2 * PA_TILE + rows_kept * HS * (int)sizeof(float))) + w * 2 * rows_kept * HS;
-        auto start_load = [&](const int (&page)[HELD], int slot) {
-            long long off[HELD];
+        // (a lane's 16-byte unit is the same one of every row that it copies)
+        const int lane_row = lane / UNITS, lane_unit = lane % UNITS;
+        const char *lane_k = (const char *)p.c.k + lane_unit * 16, *lane_v = (const char *)p.c.v + lane_unit * 16;
+        auto start_load = [&](const Rows &r, int slot) {
+            long long off[HELD];                              // in bytes; 0 for a row that does not count
+            unsigned rows[HELD];
 #pragma unroll
             for (int i = 0; i < HELD; ++i) {
-                const unsigned key = (unsigned)load.tile * KEYS + i * 32 + lane;
-                const bool ok = page[i] >= 0 && page[i] < p.c.pages;
-                off[i] = ok ? page[i] * p.c.page_stride + (key % (unsigned)p.c.page_size) * p.c.token_stride + (load.vhead / s.parts) * p.c.head_stride : -1;
-                const unsigned rows = __ballot_sync(0xffffffffu, ok);
+                const bool ok = (unsigned)r.page[i] < (unsigned)p.c.pages;
+                off[i] = ok ? (r.page[i] * p.c.page_stride + r.in_page[i] * p.c.token_stride + (load.vhead / s.parts) * p.c.head_stride) * (long long)sizeof(T) : 0;
+                rows[i] = __ballot_sync(0xffffffffu, ok);
 #pragma unroll
                 for (int j = 0; j < PA_STAGES; ++j)
-                    if (j == slot) valid[j][i] = rows;
+                    if (j == slot) valid[j][i] = rows[i];
+                rows[i] >>= lane_row;
             }
             unsigned char *k = ring + slot * 2 * PA_TILE, *v = k + PA_TILE;
 #pragma unroll
             for (int i = 0; i < PA_TILE / 512; ++i) {
-                const int lin = i * 32 + lane, row = lin / UNITS, u = lin % UNITS;
-                const long long from = HELD == 1 ? __shfl_sync(0xffffffffu, off[0], row)
-                                                 : __shfl_sync(0xffffffffu, off[i * 32 / UNITS / 32], row & 31);
-                const int place = F32 ? fm::unit_of(row, u) : UNITS >= 8 ? u ^ (row & 7) : u ^ ((row >> 1) & 3);
-                const long long el = from < 0 ? 0 : from + u * (16 / (int)sizeof(T));
-                fm::cp_async16(k + (row * UNITS + place) * 16, (const T *)p.c.k + el, from >= 0);
-                fm::cp_async16(v + (row * UNITS + place) * 16, (const T *)p.c.v + el, from >= 0);
+                constexpr int STEP = 32 / UNITS;              // rows an instruction
+                const int row = i * STEP + lane_row, held = i * STEP / 32;
+                const long long from = __shfl_sync(0xffffffffu, off[held], row & 31);
+                const bool ok = rows[held] >> (i * STEP & 31) & 1;
+                const int unit = F32 ? fm::unit_of(row, lane_unit) : UNITS >= 8 ? lane_unit ^ (row & 7) : lane_unit ^ ((row >> 1) & 3);
+                fm::cp_async16(k + (row * UNITS + unit) * 16, lane_k + from, ok);
+                fm::cp_async16(v + (row * UNITS + unit) * 16, lane_v + from, ok);
             }
             // A head's queries come with its first tile, or, where there is no room for them, on their way to L2 ahead of the reading.  Two
             // buffers: when this tile is loaded the head at hand has read its own, so only the next tile's may still have to be read.
@@ -451,26 +477,26 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
             ++done;
         };
 
-        int next_page[HELD];                                  // for the tile that is loaded next
+        Rows next_rows;                                       // of the tile that is loaded next
         {
             float x[HS / 4];
             read_queries(queries(here), x);
             heads_read ^= here.tile == 0;                     // (its first tile brings them again)
-            int page[PA_STAGES - 1][HELD];
+            Rows rows[PA_STAGES - 1];
             Place ahead = load;
             int ahead_place = load_place;
 #pragma unroll
             for (int i = 0; i < PA_STAGES - 1; ++i)
                 if (ahead_place < end) {
-                    look_up(ahead, page[i]);
+                    look_up(ahead, rows[i]);
                     ahead_place += ahead.next(s, p.lens);
                 }
 #pragma unroll
             for (int i = 0; i < PA_STAGES - 1; ++i) {
-                if (load_place < end) start_load(page[i], i);
+                if (load_place < end) start_load(rows[i], i);
                 fm::cp_commit();
             }
-            if (load_place < end) look_up(load, next_page);
+            if (load_place < end) look_up(load, next_rows);
             begin_head(x);
         }
         int slot = 0;
@@ -478,8 +504,8 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
             asm volatile("cp.async.wait_group %0;" ::"n"(PA_STAGES - 2) : "memory");
             __syncwarp();
             if (load_place < end) {
-                start_load(next_page, slot == 0 ? PA_STAGES - 1 : slot - 1);
-                if (load_place < end) look_up(load, next_page);
+                start_load(next_rows, slot == 0 ? PA_STAGES - 1 : slot - 1);
+                if (load_place < end) look_up(load, next_rows);
             }
             fm::cp_commit();
             unsigned rows[HELD];
@@ -537,27 +563,35 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
                 }
             }
             // weights
+            bool full = true;                                 // all rows count
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) full = full && rows[i] == (KEYS >= 32 ? ~0u : (1u << (KEYS & 31)) - 1);
+            if (!full)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (!(rows[i / 4] >> (8 * (i % 4) + 2 * t + e) & 1)) sc[i][e] = -INFINITY;
             float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (rows[i / 4] >> (8 * (i % 4) + 2 * t + e) & 1) top = fmaxf(top, sc[i][e]);
+            for (int i = 0; i < NT; ++i) top = fmaxf(top, fmaxf(sc[i][0], sc[i][1]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             if (__any_sync(0xffffffffu, top > m)) {
-                const float mn = fmaxf(m, top), by = m == -INFINITY ? 0.0f : exp2f((m - mn) * f);
+                const float mn = fmaxf(m, top), by = m == -INFINITY ? 0.0f : two_to((m - mn) * f);
                 l *= by;
 #pragma unroll
                 for (int i = 0; i < HS / 8; ++i) { o[i][0] *= by; o[i][1] *= by; }
                 m = mn;
             }
             const float from = m == -INFINITY ? 0.0f : m;
+            // (the weight of a row that does not count is 0 also where f is 0)
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    sc[i][e] = rows[i / 4] >> (8 * (i % 4) + 2 * t + e) & 1 ? exp2f(fmaf(sc[i][e] - from, f, SHIFT)) : 0.0f;
+                    const float x = two_to(fmaf(sc[i][e] - from, f, SHIFT));
+                    sc[i][e] = full || (rows[i / 4] >> (8 * (i % 4) + 2 * t + e) & 1) ? x : 0.0f;
                     l += sc[i][e];
                 }
             // weights times values
@@ -938,6 +972,7 @@ int bmb_paged_attention(float *out, float *lse, const float *q, const bmb_kv_cac
     p.q_stride = q_stride;
     p.out_stride = out_stride;
     p.max_pages = max_pages;
+    p.page_size = Divide((unsigned)cache->page_size);
     p.scale = scale;
     const int hs = cache->head_size, blocks = attend_blocks();
     p.s = attend_shape(n, heads, cache->heads, hs, cache->type, max_pages * cache->page_size);
