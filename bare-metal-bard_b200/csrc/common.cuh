@@ -210,6 +210,26 @@ int launch(bool in_chain, void (*kernel)(P...), dim3 grid, dim3 threads, size_t 
     count_launch();
     return BMB_OK;
 }
+// The same with blocks in clusters of `cluster`.
+template <typename... P, typename... A>
+int launch_cluster(void (*kernel)(P...), unsigned grid, int cluster, int threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = threads;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    BMB_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+    count_launch();
+    return BMB_OK;
+}
 template <typename... P, typename... A>
 int launch_in_chain(void (*kernel)(P...), dim3 grid, dim3 threads, size_t smem, cudaStream_t st, A... args) {
     return launch(true, kernel, grid, threads, smem, st, args...);

@@ -78,22 +78,28 @@ int run_write(const bmb_kv_cache &c, const float *k, const float *v, long long r
 // instruction are the 8 rows' first pieces and their second ones, so a row's two sums lie in one lane and are added there.  fp16:
 // two pieces of 11 bits, scaled by a power of two for each row of q (weights by 2^14), kept down to 2^-38 of the row's
 // largest.  bf16: three of 8 bits, the third in an instruction of its own.  fp32: two TF32 pieces (fm, flash_mma.cuh) of queries and
-// weights, and of keys and values as they are read.  Sums over tiles are kept in fp32 registers.  Masked and absent tokens are zeros in
+// weights, and of keys and values as they are read (cutting the first piece off instead of rounding it saved 1 % and lost a bit: errors of
+// 4.5e-7 in the 2-norm for 2.8e-7).  Sums over tiles are kept in fp32 registers.  Masked and absent tokens are zeros in
 // shared memory with a weight of zero, whatever the memory there holds.
 constexpr int PA_WARPS = 4, PA_THREADS = 32 * PA_WARPS, PA_STAGES = 3, PA_TILE = 4096, PA_ROWS = 8;
 constexpr int PA_BLOCKS = 2;            // blocks an SM
 constexpr int PA_MOST_BLOCKS = 512;
-// Where heads are no more than blocks and short, a block takes each head alone, a quarter of its tiles a warp: no line to find a place in
-// and no second launch, which together are 3 to 4 us; but a warp then has up to tiles / 4 of them in a row, 0.6 us each, where the line spreads
-// all over the GPU.  Measured, alone / line, at the longest length the tables hold: 6 heads of 64 fp32 of 8, 16 and 24 tiles 5.7 / 7.6,
-// 8.2 / 7.7, 10.5 / 7.8 us; 96 heads bf16 of 16 and 24 tiles 9.9 / 10.9, 13.0 / 11.7; 256 heads of 128 fp16 of 32 tiles 16.0 / 25.0.  Above
-// PA_ALONE_TILES one long request among short ones would cost too much.
-constexpr int PA_ALONE_TILES = 32;
-inline bool heads_alone(long long heads, int tiles, int blocks) {
-    return heads <= blocks && tiles <= PA_ALONE_TILES && tiles * (blocks - heads) <= 16LL * blocks;
-}
 constexpr size_t PA_SMEM = 112 * 1024;   // dynamic shared memory with which two blocks fit an SM
-
+constexpr int PA_CLUSTER = 8;
+// Blocks for each head, a cluster of them, or 0 for the line (below).  Where heads are few or short a cluster takes each alone: no line to find a
+// place in and no second launch, which together are 2 to 4 us of GPU time and 4 of the host's.  But then the longest head alone says how long it
+// takes, 0.7 us for each tile that a warp has of it, where the line spreads over all SMs.  As many blocks a head as fill the GPU (7/8 of the blocks that
+// it holds: clusters do not fill its last ones) and have a tile for each warp; and then no more tiles a warp than 2, or 8 where the blocks fill the GPU.
+// Measured, clusters / line, us, every length the longest that the tables hold: 6 heads of 64 fp32 (48 blocks) of 1, 2 and 4 tiles a warp 6.1 / 8.0,
+// 7.4 / 8.1, 10.2 / 8.5; 48 heads bf16 (192) of 2, 4 and 8 tiles 7.8 / 10.0, 10.7 / 11.8, 17.1 / 18.3; 32 heads of 128 fp16 (256) of 2, 4 and 8 tiles
+// 9.1 / 11.6, 11.6 / 15.1, 17.2 / 21.1; 288 heads bf16 of 4 and 8 tiles 11.3 / 15.9, 17.3 / 22.0.  With lengths from 1 up the line gains: 192 blocks
+// of 8 tiles 13.2 / 11.6, 288 blocks of 8 tiles 16.0 / 16.3.
+inline int blocks_alone(long long heads, int tiles, int blocks) {
+    int k = 1;
+    while (k < PA_CLUSTER && heads * 2 * k <= blocks * 7 / 8 && PA_WARPS * k < tiles) k *= 2;
+    const int each = (tiles + PA_WARPS * k - 1) / (PA_WARPS * k);
+    return heads * k <= blocks && each * (long long)blocks <= 2 * blocks + 6 * heads * k ? k : 0;
+}
 // All places in a line: requests in order, of each its (virtual) heads, of each its tiles and one place more, without work of its own, for
 // what a head costs to begin and to end (without it the runs with many short heads were the last to end: 9 heads in one of 11 tiles
 // took 31 us where the others took 24).
@@ -169,6 +175,14 @@ __device__ __forceinline__ float two_to(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long x, y, z;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(z) : "l"(x), "l"(y));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(z));
+    return a;
+}
 template <bool TRANS>
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     if (TRANS)
@@ -186,9 +200,19 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi, __half) {
 }
 __device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&v)); }
 __device__ __forceinline__ float2 unpack(uint32_t v, __half) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
-// A pair of fp32 values as pairs of pieces, the nearest value of the type each; `pieces` of them.
+// A pair of fp32 values as pairs of pieces, the nearest value of the type each (bf16, three pieces: 8 bits each, cut off, which add up exactly);
+// `pieces` of them.
 template <typename T, int pieces>
 __device__ __forceinline__ void split(float x, float y, uint32_t (&out)[pieces]) {
+    if constexpr (pieces == 3) {
+        float2 v = make_float2(x, y);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            out[i] = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
+            if (i < 2) v = add2(v, make_float2(-__uint_as_float(__float_as_uint(v.x) & 0xffff0000u), -__uint_as_float(__float_as_uint(v.y) & 0xffff0000u)));
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < pieces; ++i) {
         out[i] = pack(x, y, T());
@@ -210,6 +234,21 @@ struct Divide {
     __device__ __forceinline__ unsigned quotient(unsigned n) const { return (unsigned)(((unsigned long long)__umulhi(n, mul) + n) >> bits); }
 };
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// *p of another block of the cluster
+template <typename V>
+__device__ __forceinline__ V read_of(const float *p, unsigned rank) {
+    uint32_t a;
+    V v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    if constexpr (sizeof(V) == 16) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    else asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
 // Rows of a head in the workspace: of a block, the part of the head that it ends (0) and of the one that it begins (1).
 struct Parts {
     float *o, *m, *l;      // [blocks][2][PA_ROWS][HS], [blocks][2][PA_ROWS]
@@ -229,7 +268,7 @@ struct Attend {
     Divide page_size;
     float scale;
     bool staged, aligned_q;      // queries are staged in shared memory, 16 bytes at a time
-    bool alone;                  // a block for each head, not the line
+    int alone;                   // blocks for each head, a cluster (0: the line)
     Shape s;
     Parts w;
 };
@@ -269,12 +308,13 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
     long long begin = 0;                                      // of this warp's run in the line, and its places, from 0: the next one and the end
     int at_place = 0, end = 0;
     if (p.alone) {
-        here.request = blockIdx.x / s.vheads;
-        here.vhead = blockIdx.x - here.request * s.vheads;
+        const int head = blockIdx.x / p.alone, warp = (blockIdx.x - head * p.alone) * PA_WARPS + w, warps = p.alone * PA_WARPS;
+        here.request = head / s.vheads;
+        here.vhead = head - here.request * s.vheads;
         here.len = s.length(p.lens[here.request]);
         here.tiles = s.tiles(here.len);
-        here.tile = (int)((long long)here.tiles * w / PA_WARPS);
-        end = (int)((long long)here.tiles * (w + 1) / PA_WARPS) - here.tile;
+        here.tile = here.tiles * warp / warps;                // (few of them)
+        end = here.tiles * (warp + 1) / warps - here.tile;
         __syncthreads();
     } else {
         // how many places (of one head each) lie before each thread's stretch of requests
@@ -383,7 +423,8 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
         // pieces of its queries: 16-bit types [HS / 16][first piece, second] (+ third for bf16), fp32 [HS / 8][4]
         uint32_t qa[F32 ? 1 : HS / 16][4], ql[BF ? HS / 16 : 1][2];
         float qf[F32 ? HS / 8 : 1][4];
-        float o[HS / 8][2], m = 0.0f, l = 0.0f, f = 0.0f;     // m in units of the scores as the products give them, f: log2's of one of those
+        float2 o[HS / 8];
+        float m = 0.0f, l = 0.0f, f = 0.0f;     // m in units of the scores as the products give them, f: log2's of one of those
         bool begins = false;
         int done = 0;                                         // parts kept for joining
         // (x: a lane's elements of q, read ahead of what else waits for memory)
@@ -429,7 +470,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
                 }
             }
 #pragma unroll
-            for (int i = 0; i < HS / 8; ++i) o[i][0] = o[i][1] = 0.0f;
+            for (int i = 0; i < HS / 8; ++i) o[i] = make_float2(0.0f, 0.0f);
             m = -INFINITY;
             l = 0.0f;
             begins = here.tile == 0;
@@ -443,7 +484,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
             const float top = m * f;                          // (-inf where nothing counted; f may be 0)
             const int kept = min(PA_ROWS, s.group - (here.vhead % s.parts) * PA_ROWS);
             l *= down;
-            if (begins && ends) {
+            if (begins && ends && p.alone <= 1) {
                 if (g >= kept) return;
                 const int h = (here.vhead / s.parts) * s.group + (here.vhead % s.parts) * PA_ROWS + g;
                 float *to = p.out + here.request * p.out_stride + (long long)h * HS;
@@ -451,7 +492,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < HS / 8; ++i)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) to[column(i, e)] = o[i][e] * by;
+                    for (int e = 0; e < 2; ++e) to[column(i, e)] = (e ? o[i].y : o[i].x) * by;
                 if (p.lse && t == 0) p.lse[(size_t)here.request * s.heads + h] = l == 0.0f ? -INFINITY : fmaf(top, 0.6931471805599453f, logf(l));
                 return;
             }
@@ -464,7 +505,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < HS / 8; ++i)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) to[g * HS + column(i, e)] = o[i][e] * down;
+                    for (int e = 0; e < 2; ++e) to[g * HS + column(i, e)] = (e ? o[i].y : o[i].x) * down;
                 if (t == 0) {
                     part_m[w][done][g] = l == 0.0f ? -INFINITY : top;
                     part_l[w][done][g] = l;
@@ -472,7 +513,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
             }
             if (lane == 0) {
                 part_of[w][done] = make_int4(here.request, here.vhead, (begins ? 1 : 0) | (ends ? 2 : 0), 1);
-                if (begins) last_block[w] = line.warp_of(begin + at_place + here.tiles - 1 - here.tile) / PA_WARPS;
+                if (begins && !p.alone) last_block[w] = line.warp_of(begin + at_place + here.tiles - 1 - here.tile) / PA_WARPS;
             }
             ++done;
         };
@@ -530,10 +571,11 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
                     for (int jj = 0; jj < HS / 16; ++jj) {
                         const float4 x = fm::tile_ld<HS>(reinterpret_cast<const float *>(kt), 8 * i + g, 4 * jj + t);
                         const float4 h = make_float4(round_tf32_alu(x.x), round_tf32_alu(x.y), round_tf32_alu(x.z), round_tf32_alu(x.w));
+                        const float2 a = add2(make_float2(x.x, x.y), make_float2(-h.x, -h.y)), b = add2(make_float2(x.z, x.w), make_float2(-h.z, -h.w));
                         mma8(c[0], qf[2 * jj], h.x, h.y);
                         mma8(c[1], qf[2 * jj + 1], h.z, h.w);
-                        mma8(d[0], qf[2 * jj], x.x - h.x, x.y - h.y);
-                        mma8(d[1], qf[2 * jj + 1], x.z - h.z, x.w - h.w);
+                        mma8(d[0], qf[2 * jj], a.x, a.y);
+                        mma8(d[1], qf[2 * jj + 1], b.x, b.y);
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) sc[i][e] = (c[0][e] + c[1][e]) + ((c[0][2 + e] + c[1][2 + e]) + (d[0][e] + d[1][e]));
@@ -549,17 +591,19 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
                         const int u = 2 * jj + (id & 1);
                         uint32_t b[4];
                         ldmatrix4<false>(b, ka + (row * UNITS + (UNITS >= 8 ? u ^ (row & 7) : u ^ ((row >> 1) & 3))) * 16);
-                        mma16(c[0][jj & 1], qa[jj][0], qa[jj][1], qa[jj][2], qa[jj][3], b[0], b[1], T());
-                        mma16(c[1][jj & 1], qa[jj][0], qa[jj][1], qa[jj][2], qa[jj][3], b[2], b[3], T());
-                        if constexpr (BF) {
-                            mma16(d[0], ql[jj][0], 0, ql[jj][1], 0, b[0], b[1], T());
-                            mma16(d[1], ql[jj][0], 0, ql[jj][1], 0, b[2], b[3], T());
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            mma16(c[k][jj & 1], qa[jj][0], qa[jj][1], qa[jj][2], qa[jj][3], b[2 * k], b[2 * k + 1], T());
+                            if constexpr (BF) mma16(d[k], ql[jj][0], 0, ql[jj][1], 0, b[2 * k], b[2 * k + 1], T());
                         }
                     }
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) sc[i + k][e] = (c[k][0][e] + c[k][1][e]) + ((c[k][0][2 + e] + c[k][1][2 + e]) + d[k][e]);
+                    for (int k = 0; k < 2; ++k) {
+                        const float2 x = add2(add2(make_float2(c[k][0][0], c[k][0][1]), make_float2(c[k][1][0], c[k][1][1])),
+                                              add2(add2(make_float2(c[k][0][2], c[k][0][3]), make_float2(c[k][1][2], c[k][1][3])), make_float2(d[k][0], d[k][1])));
+                        sc[i + k][0] = x.x;
+                        sc[i + k][1] = x.y;
+                    }
                 }
             }
             // weights
@@ -581,7 +625,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
                 const float mn = fmaxf(m, top), by = m == -INFINITY ? 0.0f : two_to((m - mn) * f);
                 l *= by;
 #pragma unroll
-                for (int i = 0; i < HS / 8; ++i) { o[i][0] *= by; o[i][1] *= by; }
+                for (int i = 0; i < HS / 8; ++i) { o[i].x *= by; o[i].y *= by; }
                 m = mn;
             }
             const float from = m == -INFINITY ? 0.0f : m;
@@ -615,14 +659,13 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float ah = round_tf32_alu(a[e]), bh = round_tf32_alu(b[e]);
+                            const float2 r = add2(make_float2(a[e], b[e]), make_float2(-ah, -bh));
                             mma8(c[e], pw[i], ah, bh);
-                            mma8(c[e], pw[i], a[e] - ah, b[e] - bh);
+                            mma8(c[e], pw[i], r.x, r.y);
                         }
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) o[4 * d + e][k] += c[e][k] + c[e][2 + k];
+                    for (int e = 0; e < 4; ++e) o[4 * d + e] = add2(o[4 * d + e], add2(make_float2(c[e][0], c[e][1]), make_float2(c[e][2], c[e][3])));
                 }
             } else {
                 uint32_t pw[NT][BF ? 3 : 2];
@@ -645,9 +688,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
                         }
                     }
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) o[2 * d + k][e] += c[k][e] + c[k][2 + e];
+                    for (int k = 0; k < 2; ++k) o[2 * d + k] = add2(o[2 * d + k], add2(make_float2(c[k][0], c[k][1]), make_float2(c[k][2], c[k][3])));
                 }
             }
             const bool ends = here.tile + 1 == here.tiles, last = at_place + (ends ? 2 : 1) >= end;
@@ -696,9 +737,16 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
             }
         const unsigned firsts = __ballot_sync(0xffffffffu, first);
         if (first) group_of[__popc(firsts & ((1u << lane) - 1))] = lane | last << 8 | flags << 16;
-        if (first && flags == 1) p.w.begun[blockIdx.x] = make_int4(of.x, of.y, last_block[lane >> 1], 1);
+        if (first && flags == 1 && !p.alone) p.w.begun[blockIdx.x] = make_int4(of.x, of.y, last_block[lane >> 1], 1);
         if (lane == 0) groups = __popc(firsts);
         if (!__any_sync(0xffffffffu, first && flags == 1) && lane == 0 && !p.alone) p.w.begun[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    // (of a cluster: the block's part of the head, in the second place of the first warp's ring)
+    float *block_o = reinterpret_cast<float *>(smem + 2 * PA_TILE), *block_m = block_o + PA_ROWS * HS, *block_l = block_m + PA_ROWS;
+    static_assert(PA_ROWS * (HS + 2) * sizeof(float) <= 2 * PA_TILE, "");
+    if (p.alone > 1 && threadIdx.x < PA_ROWS) {               // (nothing, if it has no tile)
+        block_m[threadIdx.x] = -INFINITY;
+        block_l[threadIdx.x] = 0.0f;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < groups * rows_kept * (HS / 4); i += PA_THREADS) {
@@ -722,7 +770,13 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
             x[2] = use ? fmaf(v.z, by, x[2]) : x[2];
             x[3] = use ? fmaf(v.w, by, x[3]) : x[3];
         }
-        if (flags == 3) {
+        if (p.alone > 1) {
+            *reinterpret_cast<float4 *>(block_o + r * HS + d) = make_float4(x[0], x[1], x[2], x[3]);
+            if (d == 0) {
+                block_m[r] = top;
+                block_l[r] = all;
+            }
+        } else if (flags == 3) {
             float *to = p.out + of.x * p.out_stride + (long long)h * HS + d;
             const float by = all == 0.0f ? 0.0f : 1.0f / all;
 #pragma unroll
@@ -736,6 +790,43 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
                 p.w.l[row] = all;
             }
         }
+    }
+    if (p.alone > 1) {
+        // the cluster's blocks join their parts, a share of the elements each
+        cluster_sync();
+        const int head = blockIdx.x / p.alone, request = head / s.vheads, vhead = head - request * s.vheads;
+        const int kept = min(PA_ROWS, s.group - (vhead % s.parts) * PA_ROWS), h0 = (vhead / s.parts) * s.group + (vhead % s.parts) * PA_ROWS;
+        for (int i = (blockIdx.x - head * p.alone) * PA_THREADS + threadIdx.x; i < kept * (HS / 4); i += p.alone * PA_THREADS) {
+            const int r = i / (HS / 4), d = i % (HS / 4) * 4;
+            float m[PA_CLUSTER], l[PA_CLUSTER], top = -INFINITY, all = 0.0f, x[4] = {};
+            float4 v[PA_CLUSTER];
+#pragma unroll
+            for (int k = 0; k < PA_CLUSTER; ++k) {
+                m[k] = -INFINITY;
+                l[k] = 0.0f;
+                if (k >= p.alone) continue;
+                m[k] = read_of<float>(block_m + r, k);
+                l[k] = read_of<float>(block_l + r, k);
+                v[k] = read_of<float4>(block_o + r * HS + d, k);
+                top = fmaxf(top, m[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < PA_CLUSTER; ++k) {
+                if (l[k] == 0.0f) continue;
+                const float by = l[k] == l[k] ? exp2f(m[k] - top) : l[k];
+                all = fmaf(l[k], by, all);
+                x[0] = fmaf(v[k].x, by, x[0]);
+                x[1] = fmaf(v[k].y, by, x[1]);
+                x[2] = fmaf(v[k].z, by, x[2]);
+                x[3] = fmaf(v[k].w, by, x[3]);
+            }
+            float *to = p.out + request * p.out_stride + (long long)(h0 + r) * HS + d;
+            const float by = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[j] = x[j] * by;
+            if (p.lse && d == 0) p.lse[(size_t)request * s.heads + h0 + r] = all == 0.0f ? -INFINITY : fmaf(top, 0.6931471805599453f, logf(all));
+        }
+        cluster_sync();                                       // (the others have read this block's part)
     }
     // ---- requests without tokens ----
     for (int r = blockIdx.x; r < s.n; r += gridDim.x) {
@@ -856,8 +947,9 @@ int run_attend(Attend &p, cudaStream_t st) {
         BMB_CUDA(cudaFuncSetAttribute(attend_k<T, HS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PA_SMEM));
         prepared.fetch_or(bit, std::memory_order_relaxed);
     }
-    BMB_TRY(launch_in_chain(attend_k<T, HS>, p.alone ? p.s.n * p.s.vheads : blocks, PA_THREADS, least + (p.staged ? PA_WARPS * 2 * part : 0), st, p));
-    if (p.alone) return BMB_OK;
+    const size_t smem = least + (p.staged ? PA_WARPS * 2 * part : 0);
+    if (p.alone) return launch_cluster(attend_k<T, HS>, p.s.n * p.s.vheads * p.alone, p.alone, PA_THREADS, smem, st, p);
+    BMB_TRY(launch_in_chain(attend_k<T, HS>, blocks, PA_THREADS, smem, st, p));
     return launch_in_chain(attend_join_k<HS>, dim3(blocks, rows), PJ_THREADS, 0, st, p);
 }
 template <typename T>
@@ -978,7 +1070,7 @@ int bmb_paged_attention(float *out, float *lse, const float *q, const bmb_kv_cac
     p.s = attend_shape(n, heads, cache->heads, hs, cache->type, max_pages * cache->page_size);
     if ((double)n * p.s.vheads * p.s.places(p.s.cap) > 1e12)
         return fail(BMB_E_LIMIT, "paged_attention: %d requests of %d tokens", n, p.s.cap);
-    p.alone = heads_alone((long long)n * p.s.vheads, p.s.tiles(p.s.cap), blocks);
+    p.alone = blocks_alone((long long)n * p.s.vheads, p.s.tiles(p.s.cap), blocks);
     p.w.o = (float *)workspace;
     p.w.m = p.w.o + (size_t)blocks * 2 * PA_ROWS * hs;
     p.w.l = p.w.m + (size_t)blocks * 2 * PA_ROWS;

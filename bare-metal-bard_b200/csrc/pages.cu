@@ -209,26 +209,6 @@ __global__ void __launch_bounds__(THREADS) release_k(int *free_pages, int *free_
     if (me == 0 && threadIdx.x == 0) *free_out = (int)min(before, (long long)pages);
 }
 
-// BLOCKS blocks of one cluster, beside the end of the launch before.
-template <int BLOCKS, typename... P, typename... A>
-int launch_cluster(void (*kernel)(P...), int threads, cudaStream_t st, A... args) {
-    cudaLaunchAttribute at[2]{};
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = BLOCKS;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = BLOCKS;
-    cfg.blockDim = threads;
-    cfg.stream = st;
-    cfg.attrs = at;
-    cfg.numAttrs = BLOCKS > 1 ? 2 : 1;
-    BMB_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
-    count_launch();
-    return BMB_OK;
-}
-
 // Up to 256 requests and 1024 tokens (or table entries, by the tables' size): one block of 256 threads.  Up to 2048 tokens or 8192 entries: one of
 // 1024.  Beyond: a cluster of 8.  Measured, us: 64 tokens 3.0 with 256 threads, 3.9 with 1024; 1424 tokens of 256 requests 5.9, 5.0 and
 // 5.3 with the cluster; 15 thousand tokens 15.7 with 1024, 6.0 with the cluster.  Release, tables of 1024 entries 4.2 and 4.2; of 4000
@@ -259,7 +239,7 @@ int bmb_pages_assign(int *tables, int *lens_out, int *slots, int *positions, int
         return fail(BMB_E_ARG, "pages_assign: a null pointer");
     auto run = [&](auto blocks, auto threads) {
         constexpr int B = decltype(blocks)::value, N = decltype(threads)::value;
-        return launch_cluster<B>(assign_k<B, N>, N, (cudaStream_t)stream, tables, lens_out, slots, positions, owners, starts, free_left, lens, new_lens,
+        return launch_cluster(assign_k<B, N>, B, B, N, 0, (cudaStream_t)stream, tables, lens_out, slots, positions, owners, starts, free_left, lens, new_lens,
                                  free_pages, free_count, n, max_pages, page_size, pages, max_tokens);
     };
     if (n <= PG_FEW_REQUESTS && max_tokens <= PG_FEW) return run(Int<1>(), Int<256>());
@@ -273,7 +253,7 @@ int bmb_pages_release(int *free_pages, int *free_out, int *lens_out, const int *
         return fail(BMB_E_ARG, "pages_release: a null pointer");
     auto run = [&](auto blocks, auto threads) {
         constexpr int B = decltype(blocks)::value, N = decltype(threads)::value;
-        return launch_cluster<B>(release_k<B, N>, N, (cudaStream_t)stream, free_pages, free_out, lens_out, free_count, lens, tables, done, n, max_pages,
+        return launch_cluster(release_k<B, N>, B, B, N, 0, (cudaStream_t)stream, free_pages, free_out, lens_out, free_count, lens, tables, done, n, max_pages,
                                  page_size, pages);
     };
     const long long entries = (long long)n * max_pages;

@@ -520,11 +520,13 @@ def test_the_same_call_twice_gives_the_same_bits(bmb, cuda):
 
 
 @pytest.mark.parametrize("name", TYPES)
-def test_attention_with_a_block_for_each_head(bmb, cuda, name):
-    """Few and short heads, which a block each serves without a second launch, and their like beyond that form's borders."""
+def test_attention_with_blocks_for_each_head(bmb, cuda, name):
+    """Few and short heads, which a cluster of 1 to 8 blocks each serves without a second launch, and their like beyond that form's borders."""
     for hs in (32, 64, 128):
         keys = 4096 // (hs * (4 if name == "fp32" else 2))
-        for L in (1, keys, 4 * keys + 1, 15 * keys - 3, 32 * keys - 16, 33 * keys):
+        for L in (1, keys, 4 * keys + 1, 9 * keys, 15 * keys - 3, 32 * keys - 16, 33 * keys, 64 * keys + 5, 100 * keys):
             check_attention(bmb, cuda, name, "tokens", [L], 6, 3, hs, 16)
-            check_attention(bmb, cuda, name, "heads", [max(L - 7 * i, 0) for i in range(24)], 24, 12, hs, 16, bad_pages=True)
+            check_attention(bmb, cuda, name, "heads", [max(L - 7 * i, 0) for i in range(5)], 24, 12, hs, 16, bad_pages=True)
+            check_attention(bmb, cuda, name, "heads", [max(L - 7 * i, 0) for i in range(24)], 12, 12, hs, 16, lse=False)
+            check_attention(bmb, cuda, name, "interleaved", [L, 3, 0], 17, 1, hs, 24)
         check_attention(bmb, cuda, name, "tokens", [0, 5, 0], 9, 1, hs, 16)

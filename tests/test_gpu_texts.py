@@ -106,23 +106,25 @@ def test_one_text_is_what_generate_draws(bmb, cuda):
     t.close()
 
 
-def test_training_goes_on_after_texts(bmb, cuda):
-    """Drawing leaves a trainer's state alone: the same steps give the same losses with and without it."""
-    losses = []
-    for draw in (False, True):
-        t = bmb.Trainer(seed=9, max_seq_len=32, vocab_size=65, padded_vocab=128, n_layer=2, n_head=2, n_embd=64, B=2, T=32, math=bmb.MATH_FP32)
-        rng = np.random.default_rng(0)
-        got = []
-        for step in range(1, 6):
-            x = rng.integers(0, 65, (2, 33)).astype(np.int32)
-            t.upload(np.ascontiguousarray(x[:, :-1]), np.ascontiguousarray(x[:, 1:]))
-            t.step(1e-3, step)
-            if draw:
-                t.generate_batch([[1], [2, 3]], 10, seed=1, frequency=0.5)
-            got.append(t.loss())
-        losses.append(got)
-        t.close()
-    assert losses[0] == losses[1]
+def test_texts_leave_the_trainer_alone(bmb, cuda):
+    """Between two steps: parameters, gradients, the resident batch and its loss are what they were, to the bit.  (The losses of two
+    trainings cannot say so: the token embedding's gradient is added up by atomics, in another order each time.)"""
+    t = bmb.Trainer(seed=9, max_seq_len=32, vocab_size=65, padded_vocab=128, n_layer=2, n_head=2, n_embd=64, B=2, T=32, math=bmb.MATH_FP32)
+    rng = np.random.default_rng(0)
+    for step in range(1, 4):
+        x = rng.integers(0, 65, (2, 33)).astype(np.int32)
+        t.upload(np.ascontiguousarray(x[:, :-1]), np.ascontiguousarray(x[:, 1:]))
+        t.step(1e-3, step)
+        seen = []
+        for _ in range(2):
+            params, grads = np.empty(t.num_params, np.float32), np.empty(t.num_params, np.float32)
+            t.get_params(params)
+            t.get_grads(grads)
+            seen.append((params, grads, t.forward_loss()))
+            t.generate_batch([[1], [2, 3]], 10, seed=1, frequency=0.5)
+        for a, b in zip(*seen):
+            assert np.array_equal(a, b)
+    t.close()
 
 
 def test_refusals(bmb, cuda):
