@@ -5,10 +5,10 @@
 // whole text (from L2: it is short beside the row); each token found for the first time goes on a list, of which one thread each works out
 // the new value, and the pass over the part, 4 elements at a time, only picks those up.  Bound by memory where rows are many, if an element
 // that no rule touches costs few instructions: with the rules' arithmetic in the pass itself some lane of most warps needed
-// it, and 256 rows of 50257 took 41 us, the issue slots full; as it is 32.2 with all rules, of which the mask takes 2 and the biases 5 (the
-// steps between a block's barriers, which other blocks have to fill), 15.9 being what the memory takes.  Logits, mask and the first tokens and biases (not waiting for how many
-// there are) are read at once, before the counting.  Counts are whole numbers, of biases the last entry holds, and the list's order
-// does not matter, so no order of the atomics shows.
+// it, and 256 rows of 50257 took 41 us, the issue slots full.  The logits go to L2 first, while the counting waits for the text: held in registers
+// meanwhile they left room for half the blocks.  Counts are whole numbers, of biases the last entry holds, and the list's order does not
+// matter, so no order of the atomics shows.  256 rows of 50257, us: 16.3 with next to no text (15.7 being what the memory takes), 21.0 with texts of
+// up to 1024 tokens, 28.9 with 64 biases and a mask too: the steps between a block's barriers, which other blocks have to fill.
 #include "common.cuh"
 #include <climits>
 
@@ -19,10 +19,9 @@ constexpr int LG_THREADS = 256, LG_FOURS = 4, LG_PART = LG_THREADS * LG_FOURS * 
 
 // VEC: logits and out have the same offset from a 16-byte boundary, so that a row's elements can be taken 4 at a time from its first
 // boundary on: parts begin `shift` elements before multiples of LG_PART.
-// BIASES: shared memory for them, and with it 4 blocks an SM instead of 6 (256 rows of 50257 and texts of up to 1024 tokens: 22.9 us
-// without biases on 6, 26.9 on 4; with 64 biases and a mask 32.2 on 4, 34.9 where registers allow 6).
+// BIASES: shared memory for them, and with it 5 blocks an SM instead of 8.
 template <bool VEC, bool BIASES>
-__global__ void __launch_bounds__(LG_THREADS, BIASES ? 4 : 6) adjust_k(float *out, const float *logits, int V, long long stride, int parts, const __grid_constant__ bmb_logit_rules r) {
+__global__ void __launch_bounds__(LG_THREADS, BIASES ? 5 : 8) adjust_k(float *out, const float *logits, int V, long long stride, int parts, const __grid_constant__ bmb_logit_rules r) {
     // of the part, which tokens have a bias and which are in the text, a bit each; the mask's words; how often each token was drawn, and then
     // its new value; those of the text in a list; the last bias entry for each, from 1.  The last three are set up where they are used.
     constexpr int WORDS = LG_PART / 32;
@@ -45,17 +44,9 @@ __global__ void __launch_bounds__(LG_THREADS, BIASES ? 4 : 6) adjust_k(float *ou
     const float *from = logits + row * stride;
     const int v0 = (blockIdx.x - row * parts) * LG_PART - (VEC ? (int)((uintptr_t)from >> 2 & 3) : 0);      // (at most 3 before the row's first)
     const bool inner = VEC && v0 >= 0 && v0 + LG_PART <= V;
-    float x[LG_FOURS][4];
-#pragma unroll
-    for (int k = 0; k < LG_FOURS; ++k) {
-        const int v = v0 + 4 * (threadIdx.x + k * LG_THREADS);
-        if (inner || (VEC && v >= 0 && v + 3 < V)) {
-            *reinterpret_cast<float4 *>(x[k]) = *reinterpret_cast<const float4 *>(from + v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[k][e] = v + e >= 0 && v + e < V ? from[v + e] : 0.0f;
-        }
-    }
+    // the part on its way to L2, 128 bytes a thread
+    for (int v = v0 + 32 * (int)threadIdx.x; v < min(v0 + LG_PART, V); v += 32 * LG_THREADS)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(from + max(v, 0)));
     const int *text = r.history + (size_t)row * r.history_stride, *ids = r.bias_ids + (size_t)row * r.bias_stride;
     int4 token;
     int id = -1, len = 0, prompt = 0, biases = 0;
@@ -141,11 +132,23 @@ __global__ void __launch_bounds__(LG_THREADS, BIASES ? 4 : 6) adjust_k(float *ou
             const float y = seen[at >> 5] & bit(at) ? penalised(at) : from[v0 + at];
             value[at] = __fadd_rn(y, j < LG_THREADS ? bias : r.bias[(size_t)row * r.bias_stride + j]);
         });
-        for (int i = threadIdx.x; i < listed; i += LG_THREADS)
+        // (from the last thread down: the warps that have no bias first)
+        for (int i = LG_THREADS - 1 - threadIdx.x; i < listed; i += LG_THREADS)
             if (!(with_bias[list[i] >> 5] & bit(list[i]))) value[list[i]] = penalised(list[i]);
         __syncthreads();
     }
     float *to = out + row * stride;
+    float x[LG_FOURS][4];
+#pragma unroll
+    for (int k = 0; k < LG_FOURS; ++k) {
+        const int v = v0 + 4 * (threadIdx.x + k * LG_THREADS);
+        if (inner || (VEC && v >= 0 && v + 3 < V)) {
+            *reinterpret_cast<float4 *>(x[k]) = *reinterpret_cast<const float4 *>(from + v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[k][e] = v + e >= 0 && v + e < V ? from[v + e] : 0.0f;
+        }
+    }
 #pragma unroll
     for (int k = 0; k < LG_FOURS; ++k) {
         const int i = 4 * (threadIdx.x + k * LG_THREADS), v = v0 + i;
