@@ -7,8 +7,8 @@
 // that no rule touches costs few instructions: with the rules' arithmetic in the pass itself some lane of most warps needed
 // it, and 256 rows of 50257 took 41 us, the issue slots full.  The logits go to L2 first, while the counting waits for the text: held in registers
 // meanwhile they left room for half the blocks.  Counts are whole numbers, of biases the last entry holds, and the list's order does not
-// matter, so no order of the atomics shows.  256 rows of 50257, us: 16.3 with next to no text (15.7 being what the memory takes), 21.0 with texts of
-// up to 1024 tokens, 28.9 with 64 biases and a mask too: the steps between a block's barriers, which other blocks have to fill.
+// matter, so no order of the atomics shows.  256 rows of 50257, us: 17.1 with next to no text (15.7 being what the memory takes), 20.8 with texts of
+// up to 1024 tokens, 28.4 with 64 biases and a mask too: the steps between a block's barriers, which other blocks have to fill.
 #include "common.cuh"
 #include <climits>
 
@@ -23,7 +23,7 @@ constexpr int LG_THREADS = 256, LG_FOURS = 4, LG_PART = LG_THREADS * LG_FOURS * 
 template <bool VEC, bool BIASES>
 __global__ void __launch_bounds__(LG_THREADS, BIASES ? 5 : 8) adjust_k(float *out, const float *logits, int V, long long stride, int parts, const __grid_constant__ bmb_logit_rules r) {
     // of the part, which tokens have a bias and which are in the text, a bit each; the mask's words; how often each token was drawn, and then
-    // its new value; those of the text in a list; the last bias entry for each, from 1.  The last three are set up where they are used.
+    // its new value; those of the text in a list; the last bias entry for each, from 1.
     constexpr int WORDS = LG_PART / 32;
     extern __shared__ __align__(16) unsigned shared[];
     __shared__ unsigned with_bias[WORDS], seen[WORDS], mask[WORDS + 2];
@@ -32,9 +32,14 @@ __global__ void __launch_bounds__(LG_THREADS, BIASES ? 5 : 8) adjust_k(float *ou
     float *value = reinterpret_cast<float *>(shared);
     unsigned short *list = reinterpret_cast<unsigned short *>(count + LG_PART);
     int *last = reinterpret_cast<int *>(list + LG_PART);      // (only where there are biases)
-    const bool ruled = r.history || BIASES;
+    bool ruled = r.history || BIASES;
     if (ruled) {
         for (int i = threadIdx.x; i < WORDS; i += LG_THREADS) with_bias[i] = seen[i] = 0;
+#pragma unroll
+        for (int k = 0; k < LG_FOURS; ++k) {
+            reinterpret_cast<int4 *>(count)[threadIdx.x + k * LG_THREADS] = make_int4(0, 0, 0, 0);
+            if (BIASES) reinterpret_cast<int4 *>(last)[threadIdx.x + k * LG_THREADS] = make_int4(0, 0, 0, 0);
+        }
         if (threadIdx.x == 0) listed = 0;
     }
     static_assert(LG_PART <= 1 << 16, "");
@@ -83,41 +88,42 @@ __global__ void __launch_bounds__(LG_THREADS, BIASES ? 5 : 8) adjust_k(float *ou
         for (int i = threadIdx.x; i < WORDS + 2; i += LG_THREADS)
             mask[i] = w0 + i >= 0 && 32 * (w0 + i) < V ? r.allowed[(size_t)row * r.allowed_stride + w0 + i] : 0u;
     __syncthreads();
+    // the part's tokens: `span` of them from `least` on
+    const int least = max(v0, 0);
+    const unsigned span = max(min(v0 + LG_PART, V) - least, 0);      // (the last part may begin behind the row)
+    const auto bit = [](int at) { return 1u << (at & 31); };
+    // use(place in the part, index) of each bias that the part has
+    auto entries = [&](auto &&use) {
+        if (!BIASES) return;
+        for (int j = threadIdx.x; j < biases; j += LG_THREADS) {
+            const int v = j < LG_THREADS ? id : ids[j];
+            if ((unsigned)v - (unsigned)least < span) use(v - v0, j);
+        }
+    };
     if (ruled) {
-        const auto bit = [](int at) { return 1u << (at & 31); };
         len = min(max(len, 0), r.history_stride);
         biases = min(max(biases, 0), r.bias_stride);
-        // use(place in the part, index) of each token of the text, and of each bias, that the part has
-        bool first = true;
-        auto tokens = [&](auto &&use) {
-            for (int j = 4 * threadIdx.x; j < len; j += 4 * LG_THREADS) {
-                if (!first) read_text(j, len);
-                const int t[4] = {token.x, token.y, token.z, token.w};
+        bool found = false;
+        for (int j = 4 * threadIdx.x; j < len; j += 4 * LG_THREADS) {
+            if (j >= 4 * LG_THREADS) read_text(j, len);
+            const int t[4] = {token.x, token.y, token.z, token.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (t[e] >= 0 && t[e] < V && (unsigned)(t[e] - v0) < (unsigned)LG_PART && j + e < len) use(t[e] - v0, j + e);
-                first = len <= 4 * LG_THREADS;                // (they are still at hand)
+            for (int e = 0; e < 4; ++e) {
+                if ((unsigned)t[e] - (unsigned)least >= span || j + e >= len) continue;
+                const int at = t[e] - v0;
+                found = true;
+                if (j + e >= prompt) atomicAdd(&count[at], 1);
+                if (!(atomicOr(&seen[at >> 5], bit(at)) & bit(at))) list[atomicAdd(&listed, 1)] = (unsigned short)at;
             }
-        };
-        auto entries = [&](auto &&use) {
-            if (!BIASES) return;
-            for (int j = threadIdx.x; j < biases; j += LG_THREADS) {
-                const int v = j < LG_THREADS ? id : ids[j];
-                if (v >= 0 && v < V && (unsigned)(v - v0) < (unsigned)LG_PART) use(v - v0, j);
-            }
-        };
-        tokens([&](int at, int) {
-            if (atomicOr(&seen[at >> 5], bit(at)) & bit(at)) return;
-            list[atomicAdd(&listed, 1)] = (unsigned short)at;
-            count[at] = 0;
+        }
+        entries([&](int at, int j) {
+            found = true;
+            atomicMax(&last[at], j + 1);
+            atomicOr(&with_bias[at >> 5], bit(at));
         });
-        entries([&](int at, int) {
-            if (!(atomicOr(&with_bias[at >> 5], bit(at)) & bit(at))) last[at] = 0;
-        });
-        __syncthreads();
-        tokens([&](int at, int j) { if (j >= prompt) atomicAdd(&count[at], 1); });
-        entries([&](int at, int j) { atomicMax(&last[at], j + 1); });
-        __syncthreads();
+        ruled = __syncthreads_or(found);                      // (nothing: the rest is a copy)
+    }
+    if (ruled) {
         // those with a bias by the thread of its last entry, the others of the text from the list
         auto penalised = [&](int at) {
             const int drawn = count[at];

@@ -211,14 +211,14 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&out)[pieces])
             out[i] = __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
             if (i < 2) v = add2(v, make_float2(-__uint_as_float(__float_as_uint(v.x) & 0xffff0000u), -__uint_as_float(__float_as_uint(v.y) & 0xffff0000u)));
         }
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < pieces; ++i) {
-        out[i] = pack(x, y, T());
-        const float2 v = unpack(out[i], T());
-        x -= v.x;
-        y -= v.y;
+        for (int i = 0; i < pieces; ++i) {
+            out[i] = pack(x, y, T());
+            const float2 v = unpack(out[i], T());
+            x -= v.x;
+            y -= v.y;
+        }
     }
 }
 
