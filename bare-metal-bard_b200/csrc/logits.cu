@@ -94,8 +94,7 @@ __global__ void __launch_bounds__(LG_THREADS, BIASES ? 5 : 8) adjust_k(float *ou
     const auto bit = [](int at) { return 1u << (at & 31); };
     // use(place in the part, index) of each bias that the part has
     auto entries = [&](auto &&use) {
-        if (!BIASES) return;
-        for (int j = threadIdx.x; j < biases; j += LG_THREADS) {
+        for (int j = threadIdx.x; BIASES && j < biases; j += LG_THREADS) {
             const int v = j < LG_THREADS ? id : ids[j];
             if ((unsigned)v - (unsigned)least < span) use(v - v0, j);
         }

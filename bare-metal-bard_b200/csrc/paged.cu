@@ -71,7 +71,8 @@ int run_write(const bmb_kv_cache &c, const float *k, const float *v, long long r
 // Work: the tiles of all requests and cache heads stand in one line, a tile being 4 KB of keys and 4 KB of values, and are cut
 // into equal runs, one for each warp of the GPU.  A warp is on its own: its tiles come by cp.async through a ring of its own, over the
 // borders of heads and requests, and no block-wide barrier stands in the loop.  Heads that lie in several runs are joined, first
-// among the warps of a block, and what reaches over blocks by attend_join_k.  Nothing depends on arrival, so equal calls give equal bits.
+// among the warps of a block, and what reaches over blocks by attend_join_k.  Few or short heads go to a cluster of blocks each instead
+// (blocks_alone).  Nothing depends on arrival, so equal calls give equal bits.
 //
 // Arithmetic: warp-level matrix instructions, 8 query heads of one cache head a time, at fp32 accuracy.  Queries and weights are
 // fp32, so each goes in as pieces of the cache's type, whose products with its elements are exact: the 16 rows of an
@@ -81,11 +82,16 @@ int run_write(const bmb_kv_cache &c, const float *k, const float *v, long long r
 // weights, and of keys and values as they are read (cutting the first piece off instead of rounding it saved 1 % and lost a bit: errors of
 // 4.5e-7 in the 2-norm for 2.8e-7).  Sums over tiles are kept in fp32 registers.  Masked and absent tokens are zeros in
 // shared memory with a weight of zero, whatever the memory there holds.
+//
+// Bound by, and measured (us, caches cold): 609 MB of fp16, 8 requests of up to 32768 tokens, 32 heads on 8 of 128: 100, 6.1 TB/s, the loads.  203 MB of
+// fp32, 37 of up to 2777, 16 heads on 4 of 128: 44.5, and 101 MB of bf16, 64 of up to 1024, 12 heads of 64: 26.8: the loads alone take 40.7 and
+// 24.6 of that, at 6.2 TB/s behind 4 us before the first tile is there and in front of 4 for the last warps and the joins; the arithmetic alone nearly as
+// long (8 warps an SM, issue slots 43 and 34 % in use; with 12 warps and shorter rings 1 to 4 us more).
 constexpr int PA_WARPS = 4, PA_THREADS = 32 * PA_WARPS, PA_STAGES = 3, PA_TILE = 4096, PA_ROWS = 8;
-constexpr int PA_BLOCKS = 2;            // blocks an SM
-constexpr int PA_MOST_BLOCKS = 512;
-constexpr size_t PA_SMEM = 112 * 1024;   // dynamic shared memory with which two blocks fit an SM
+constexpr int PA_BLOCKS = 2, PA_MOST_BLOCKS = 512;          // blocks an SM, and in all
+constexpr size_t PA_SMEM = 112 * 1024;                       // dynamic shared memory with which two blocks fit an SM
 constexpr int PA_CLUSTER = 8;
+
 // Blocks for each head, a cluster of them, or 0 for the line (below).  Where heads are few or short a cluster takes each alone: no line to find a
 // place in and no second launch, which together are 2 to 4 us of GPU time and 4 of the host's.  But then the longest head alone says how long it
 // takes, 0.7 us for each tile that a warp has of it, where the line spreads over all SMs.  As many blocks a head as fill the GPU (7/8 of the blocks that
@@ -100,6 +106,7 @@ inline int blocks_alone(long long heads, int tiles, int blocks) {
     const int each = (tiles + PA_WARPS * k - 1) / (PA_WARPS * k);
     return heads * k <= blocks && each * (long long)blocks <= 2 * blocks + 6 * heads * k ? k : 0;
 }
+
 // All places in a line: requests in order, of each its (virtual) heads, of each its tiles and one place more, without work of its own, for
 // what a head costs to begin and to end (without it the runs with many short heads were the last to end: 9 heads in one of 11 tiles
 // took 31 us where the others took 24).
@@ -190,15 +197,10 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     else
         asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
 __device__ __forceinline__ uint32_t pack(float lo, float hi, __half) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
-__device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&v)); }
 __device__ __forceinline__ float2 unpack(uint32_t v, __half) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
 // A pair of fp32 values as pairs of pieces, the nearest value of the type each (bf16, three pieces: 8 bits each, cut off, which add up exactly);
 // `pieces` of them.
