@@ -106,6 +106,12 @@ int sm_count();
 void count_launch(int n = 1);
 long long launches_total();
 
+// All of these addresses are multiples of 4 (or null).
+template <typename... P>
+bool words(const P *...p) {
+    return ((... | (uintptr_t)p) & 3) == 0;
+}
+
 inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // Internal flag of gemm_any_bias: the launches of a captured stream may use the per-device scratch, because the caller

@@ -193,7 +193,8 @@ extern "C" int bmb_logits_adjust(float *out, const float *logits, int n, int V, 
     if (!rules || n < 0 || V < 0 || stride < V) return fail(BMB_E_ARG, "logits_adjust: bad argument (n=%d V=%d stride=%lld)", n, V, stride);
     if (n == 0 || V == 0) return BMB_OK;
     const bmb_logit_rules &r = *rules;
-    if (!out || !logits || (((uintptr_t)out | (uintptr_t)logits) & 3)) return fail(BMB_E_ARG, "logits_adjust: a null or unaligned pointer");
+    if (!out || !logits || !words(out, logits, r.history, r.history_lens, r.prompt_lens, r.repetition, r.frequency, r.presence, r.bias_ids, r.bias, r.bias_lens, r.allowed))
+        return fail(BMB_E_ARG, "logits_adjust: a null or unaligned pointer");
     if (!r.history && (r.repetition || r.frequency || r.presence)) return fail(BMB_E_ARG, "logits_adjust: penalties need a history");
     if (r.history && (!r.history_lens || r.history_stride < 0)) return fail(BMB_E_ARG, "logits_adjust: a history needs history_lens and a stride");
     if (!r.bias_ids != !r.bias || (r.bias_ids && (!r.bias_lens || r.bias_stride < 0)))

@@ -84,9 +84,9 @@ int run_write(const bmb_kv_cache &c, const float *k, const float *v, long long r
 // shared memory with a weight of zero, whatever the memory there holds.
 //
 // Bound by, and measured (us, caches cold): 609 MB of fp16, 8 requests of up to 32768 tokens, 32 heads on 8 of 128: 100, 6.1 TB/s, the loads.  203 MB of
-// fp32, 37 of up to 2777, 16 heads on 4 of 128: 44.5, and 101 MB of bf16, 64 of up to 1024, 12 heads of 64: 26.8: the loads alone take 40.7 and
-// 24.6 of that, at 6.2 TB/s behind 4 us before the first tile is there and in front of 4 for the last warps and the joins; the arithmetic alone nearly as
-// long (8 warps an SM, issue slots 43 and 34 % in use; with 12 warps and shorter rings 1 to 4 us more).
+// fp32, 37 of up to 2777, 16 heads on 4 of 128: 44.5, and 101 MB of bf16, 64 of up to 1024, 12 heads of 64: 26.8: the loads alone take 40.8 and
+// 24.6 of that, at 6.2 TB/s behind 4 us before the first tile is there and in front of 4 for the last warps and the joins; the arithmetic alone 43.3
+// and 24.5 (8 warps an SM, issue slots 43 and 34 % in use; with 12 warps and shorter rings 1 to 4 us more in all).
 constexpr int PA_WARPS = 4, PA_THREADS = 32 * PA_WARPS, PA_STAGES = 3, PA_TILE = 4096, PA_ROWS = 8;
 constexpr int PA_BLOCKS = 2, PA_MOST_BLOCKS = 512;          // blocks an SM, and in all
 constexpr size_t PA_SMEM = 112 * 1024;                       // dynamic shared memory with which two blocks fit an SM
@@ -974,7 +974,7 @@ int bmb_paged_kv_write(const bmb_kv_cache *cache, const float *k, const float *v
     BMB_TRY(check_cache("paged_kv_write", cache));
     if (tokens < 0 || row_stride < 0) return fail(BMB_E_ARG, "paged_kv_write: tokens=%d row_stride=%lld", tokens, row_stride);
     if (tokens == 0) return BMB_OK;
-    if (!k || !v || !slots || ((uintptr_t)k | (uintptr_t)v) & 3) return fail(BMB_E_ARG, "paged_kv_write: a null or unaligned pointer");
+    if (!k || !v || !slots || !words(k, v, slots)) return fail(BMB_E_ARG, "paged_kv_write: a null or unaligned pointer");
     cudaStream_t st = (cudaStream_t)stream;
     if (cache->type == BMB_TYPE_FP32) return run_write<float>(*cache, k, v, row_stride, slots, tokens, st);
     if (cache->type == BMB_TYPE_BF16) return run_write<__nv_bfloat16>(*cache, k, v, row_stride, slots, tokens, st);
@@ -1052,7 +1052,7 @@ int bmb_paged_attention(float *out, float *lse, const float *q, const bmb_kv_cac
         return fail(BMB_E_LIMIT, "paged_attention: %d pages of %d tokens are beyond an int", max_pages, cache->page_size);
     if ((long long)n * heads > INT_MAX) return fail(BMB_E_LIMIT, "paged_attention: %d requests of %d heads", n, heads);
     if (n == 0) return BMB_OK;
-    if (!out || !q || !tables || !lens || (((uintptr_t)out | (uintptr_t)q) & 3)) return fail(BMB_E_ARG, "paged_attention: a null or unaligned pointer");
+    if (!out || !q || !tables || !lens || !words(out, lse, q, tables, lens)) return fail(BMB_E_ARG, "paged_attention: a null or unaligned pointer");
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < bmb_paged_attention_workspace(heads, cache->heads, cache->head_size))
         return fail(BMB_E_ARG, "paged_attention: a workspace of %zu bytes, 16-byte aligned, is needed (got %zu)",
                     bmb_paged_attention_workspace(heads, cache->heads, cache->head_size), workspace_bytes);

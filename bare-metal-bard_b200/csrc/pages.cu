@@ -7,13 +7,14 @@
 // of them: one block.  Many: a cluster of 8, each of which counts all requests and takes an eighth of the tokens or entries; lengths are
 // read by all before any is overwritten, which a cluster's barrier can say and a grid cannot.
 #include "common.cuh"
+#include <atomic>
 #include <climits>
 #include <type_traits>
 
 namespace bmb {
 namespace {
 
-constexpr int PG_CLUSTER = 8, PG_MOST = 1024;
+constexpr int PG_CLUSTER = 8, PG_MOST = 1024, PG_STASH = 192 * 1024;
 template <int V> using Int = std::integral_constant<int, V>;
 
 __device__ __forceinline__ unsigned cluster_rank() {
@@ -141,7 +142,8 @@ __global__ void __launch_bounds__(THREADS) assign_k(int *tables, int *lens_out, 
 
 template <int BLOCKS, int THREADS>
 __global__ void __launch_bounds__(THREADS) release_k(int *free_pages, int *free_out, int *lens_out, const int *free_count, const int *lens,
-                                                     const int *tables, const int *done, int n, int max_pages, int page_size, int pages) {
+                                                     const int *tables, const int *done, int n, int max_pages, int page_size, int pages, int stash) {
+    extern __shared__ int stashed[];                          // [warps][stash]: a warp's entries, if it has no more than that
     __shared__ long long sums[2][THREADS / 32];
     __shared__ long long end_of[THREADS];                     // where the entries of the stretch's requests end
     __shared__ long long found;                               // pages of the pool among this block's entries
@@ -158,11 +160,14 @@ __global__ void __launch_bounds__(THREADS) release_k(int *free_pages, int *free_
         end_of[threadIdx.x] = block_scan<THREADS>(ends ? min(pages_of(L, page_size), max_pages) : 0, sums[0], &entries);
         sync_all<BLOCKS>();                                   // as in assign_k
         if (me == 0 && i < n) lens_out[i] = ends ? 0 : L;
-        // a run of entries for each warp, in order; once to count and once to write
+        // A run of entries for each warp, in order; once to count and once to write, the second time from shared memory where there is room
+        // (100 thousand entries read twice: 13.2 us, once: 10.2).
         constexpr int WARPS = BLOCKS * THREADS / 32, AHEAD = 4;
         const long long each = (entries + WARPS * 32 - 1) / (WARPS * 32) * 32;
         const long long from = (me * (THREADS / 32) + w) * each, to = min(from + each, entries);
-        auto walk = [&](auto &&use) {
+        const bool kept = each <= stash;
+        int *mine_stashed = stashed + w * stash;
+        auto read = [&](auto &&use) {
             int r = 0;
             if (from < to)
 #pragma unroll
@@ -180,11 +185,14 @@ __global__ void __launch_bounds__(THREADS) release_k(int *free_pages, int *free_
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) use(page[k], __ballot_sync(0xffffffffu, page[k] >= 0 && page[k] < pages));
+                for (int k = 0; k < AHEAD; ++k) {
+                    if (kept && f + 32 * k < to) mine_stashed[f + 32 * k - from] = page[k];
+                    use(page[k]);
+                }
             }
         };
         int mine = 0;
-        walk([&](int, unsigned ok) { mine += __popc(ok); });
+        read([&](int page) { mine += __popc(__ballot_sync(0xffffffffu, (unsigned)page < (unsigned)pages)); });
         long long at = block_scan<THREADS>(lane == 31 ? mine : 0, sums[1], &all) - (lane == 31 ? mine : 0);
         at = before + __shfl_sync(0xffffffffu, at, 31);
         if (BLOCKS > 1) {
@@ -197,11 +205,18 @@ __global__ void __launch_bounds__(THREADS) release_k(int *free_pages, int *free_
                 if (b < me) at += x;
             }
         }
-        walk([&](int page, unsigned ok) {
+        auto write = [&](int page) {
+            const unsigned ok = __ballot_sync(0xffffffffu, (unsigned)page < (unsigned)pages);
             const long long place = at + __popc(ok & ((1u << lane) - 1));
             if ((ok >> lane & 1) && place < pages) free_pages[place] = page;
             at += __popc(ok);
-        });
+        };
+        if (kept) {
+            const int count = (int)max(to - from, 0LL);
+            for (int i = lane; i - lane < count; i += 32) write(i < count ? mine_stashed[i] : -1);
+        } else {
+            read(write);
+        }
         before += all;
         sync_all<BLOCKS>();                                   // (the others have read `found`)
     }
@@ -211,8 +226,8 @@ __global__ void __launch_bounds__(THREADS) release_k(int *free_pages, int *free_
 
 // Up to 256 requests and 1024 tokens (or table entries, by the tables' size): one block of 256 threads.  Up to 2048 tokens or 8192 entries: one of
 // 1024.  Beyond: a cluster of 8.  Measured, us: 64 tokens 3.0 with 256 threads, 3.9 with 1024; 1424 tokens of 256 requests 5.9, 5.0 and
-// 5.3 with the cluster; 15 thousand tokens 15.7 with 1024, 6.0 with the cluster.  Release, tables of 1024 entries 4.2 and 4.2; of 4000
-// 7.3, 5.3 and 7.2; of 62 thousand 13.5 with 1024 and 7.9 with the cluster.
+// 5.3 with the cluster; 15 thousand tokens 15.7 with 1024, 6.0 with the cluster.  Release (its entries
+// read twice) from tables of 1024 entries 4.2 and 4.2; of 4000 7.3, 5.3 and 7.2; of 62 thousand 13.5 with 1024 and 7.9 with the cluster.
 constexpr int PG_FEW_REQUESTS = 256, PG_FEW = 1024, PG_SOME_TOKENS = 2048, PG_SOME_ENTRIES = 8192;
 
 int check_pool(const char *what, int n, int max_pages, int page_size, int pages) {
@@ -237,6 +252,8 @@ int bmb_pages_assign(int *tables, int *lens_out, int *slots, int *positions, int
     if (max_tokens < 0) return fail(BMB_E_ARG, "pages_assign: max_tokens=%d", max_tokens);
     if (!free_left || !free_count || (pages && !free_pages) || (max_tokens && !slots) || (n && (!tables || !lens_out || !lens || !new_lens)))
         return fail(BMB_E_ARG, "pages_assign: a null pointer");
+    if (!words(tables, lens_out, slots, positions, owners, starts, free_left, lens, new_lens, free_pages, free_count))
+        return fail(BMB_E_ARG, "pages_assign: an unaligned pointer");
     auto run = [&](auto blocks, auto threads) {
         constexpr int B = decltype(blocks)::value, N = decltype(threads)::value;
         return launch_cluster(assign_k<B, N>, B, B, N, 0, (cudaStream_t)stream, tables, lens_out, slots, positions, owners, starts, free_left, lens, new_lens,
@@ -251,12 +268,23 @@ int bmb_pages_release(int *free_pages, int *free_out, int *lens_out, const int *
     BMB_TRY(check_pool("pages_release", n, max_pages, page_size, pages));
     if (!free_out || !free_count || (pages && !free_pages) || (n && (!tables || !lens_out || !lens || !done)))
         return fail(BMB_E_ARG, "pages_release: a null pointer");
-    auto run = [&](auto blocks, auto threads) {
-        constexpr int B = decltype(blocks)::value, N = decltype(threads)::value;
-        return launch_cluster(release_k<B, N>, B, B, N, 0, (cudaStream_t)stream, free_pages, free_out, lens_out, free_count, lens, tables, done, n, max_pages,
-                                 page_size, pages);
-    };
+    if (!words(free_pages, free_out, lens_out, free_count, lens, tables, done)) return fail(BMB_E_ARG, "pages_release: an unaligned pointer");
     const long long entries = (long long)n * max_pages;
+    auto run = [&](auto blocks, auto threads) -> int {
+        constexpr int B = decltype(blocks)::value, N = decltype(threads)::value, MOST = PG_STASH / (N / 32) / 4;
+        // what a warp may have at most, if that fits
+        const long long each = (entries + B * N - 1) / (B * N) * 32;
+        const int stash = each <= MOST ? (int)each : 0;
+        static std::atomic<unsigned long long> prepared{0};       // devices (those from 64 on are prepared every time)
+        const int dev = current_device();
+        const unsigned long long bit = dev >= 0 && dev < 64 ? 1ULL << dev : 0;
+        if (!(prepared.load(std::memory_order_relaxed) & bit)) {
+            BMB_CUDA(cudaFuncSetAttribute(release_k<B, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, PG_STASH));
+            prepared.fetch_or(bit, std::memory_order_relaxed);
+        }
+        return launch_cluster(release_k<B, N>, B, B, N, (size_t)stash * (N / 32) * sizeof(int), (cudaStream_t)stream, free_pages, free_out, lens_out, free_count,
+                              lens, tables, done, n, max_pages, page_size, pages, stash);
+    };
     if (n <= PG_FEW_REQUESTS && entries <= PG_FEW) return run(Int<1>(), Int<256>());
     return entries <= PG_SOME_ENTRIES ? run(Int<1>(), Int<PG_MOST>()) : run(Int<PG_CLUSTER>(), Int<PG_MOST>());
 }

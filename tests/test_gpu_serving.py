@@ -99,7 +99,8 @@ def run_release(bmb, torch, stack, free, lens, tables, done, page, pages, in_pla
 
 @pytest.mark.parametrize("n,page,longest,share,in_place", [(1, 16, 200, 1.0, False), (5, 1, 70, 0.5, True), (64, 16, 1024, 0.25, False),
                                                             (200, 24, 3001, 0.8, True), (1023, 8, 99, 0.5, False), (1030, 16, 300, 1.0, True),
-                                                            (2100, 128, 400, 0.3, False), (40, 16, 50000, 0.6, False)])
+                                                            (2100, 128, 400, 0.3, False), (40, 16, 50000, 0.6, False),
+                                                            (300, 16, 30000, 0.9, True), (3, 1, 200000, 1.0, False)])
 def test_release(bmb, cuda, n, page, longest, share, in_place):
     rng = np.random.default_rng(n + page)
     lens = rng.integers(-3, longest + 1, n)
@@ -479,10 +480,12 @@ def test_steps_together(bmb, cuda, name, heads, kv, hs, page, pages):
     simulate(bmb, cuda, lambda: s.step(cuda.cuda.current_stream().cuda_stream), s, [[] for _ in range(9)], 30, 5)
 
 
-def test_a_captured_step_follows_the_lengths(bmb, cuda):
-    """One graph of a whole step, replayed while texts begin, grow and end: nothing of its shape came from the host."""
+@pytest.mark.parametrize("width", [15, 800])
+def test_a_captured_step_follows_the_lengths(bmb, cuda, width):
+    """One graph of a whole step, replayed while texts begin, grow and end: nothing of its shape came from the host.  (Tables for short
+    texts, and for long ones, whose attention is divided over the GPU.)"""
     torch = cuda
-    s = Serving(bmb, torch, 9, 6, 2, 64, 8, 70, 15, 200)
+    s = Serving(bmb, torch, 9, 6, 2, 64, 8, 70, width, 200)
     side = torch.cuda.Stream()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.stream(side):

@@ -34,7 +34,7 @@ def test_bad_caches_are_refused(bmb, change, code):
 @pytest.mark.parametrize("at,value,code", [
     (0, None, "E_ARG"), (2, None, "E_ARG"), (3, None, "E_ARG"), (4, None, "E_ARG"), (5, None, "E_ARG"), (6, -1, "E_ARG"), (7, 3, "E_ARG"), (7, 0, "E_ARG"),
     (8, -1, "E_ARG"), (9, 127, "E_ARG"), (10, 0, "E_ARG"), (10, 1 << 28, "E_LIMIT"), (12, None, "E_ARG"), (12, P + 8, "E_ARG"), (13, 0, "E_ARG"),
-    (6, (1 << 31) - 1, "E_LIMIT"), (0, P + 2, "E_ARG"), (2, P + 1, "E_ARG"),
+    (6, (1 << 31) - 1, "E_LIMIT"), (0, P + 2, "E_ARG"), (1, P + 2, "E_ARG"), (2, P + 1, "E_ARG"), (4, P + 2, "E_ARG"), (5, P + 3, "E_ARG"),
 ])
 def test_attention_refuses(bmb, at, value, code):
     args = [P, P, P, cache(bmb), P, P, 1, 2, 384, 128, 4, 0.125, P, 1 << 24, None]
@@ -48,7 +48,7 @@ def test_attention_of_no_requests_is_nothing(bmb):
     assert bmb.lib().bmb_paged_kv_write(cache(bmb), None, None, 384, None, 0, None) == 0
 
 
-@pytest.mark.parametrize("at,value", [(1, None), (2, None), (3, -1), (4, None), (5, -1), (1, P + 2)])
+@pytest.mark.parametrize("at,value", [(1, None), (2, None), (3, -1), (4, None), (5, -1), (1, P + 2), (4, P + 2)])
 def test_write_refuses(bmb, at, value):
     args = [cache(bmb), P, P, 384, P, 4, None]
     args[at] = value
@@ -59,7 +59,7 @@ def test_write_refuses(bmb, at, value):
     (0, None, "E_ARG"), (1, None, "E_ARG"), (2, None, "E_ARG"), (6, None, "E_ARG"), (7, None, "E_ARG"), (8, None, "E_ARG"), (9, None, "E_ARG"),
     (10, None, "E_ARG"), (11, -1, "E_ARG"), (12, 0, "E_ARG"), (13, 0, "E_ARG"), (14, -1, "E_ARG"), (15, -1, "E_ARG"), (14, 1 << 28, "E_LIMIT"),
     (12, 1 << 28, "E_LIMIT"),
-])
+] + [(i, P + 2, "E_ARG") for i in range(11)])
 def test_assign_refuses(bmb, at, value, code):
     args = [P] * 11 + [4, 8, 16, 32, 64, None]
     args[at] = value
@@ -69,7 +69,7 @@ def test_assign_refuses(bmb, at, value, code):
 @pytest.mark.parametrize("at,value,code", [
     (0, None, "E_ARG"), (1, None, "E_ARG"), (2, None, "E_ARG"), (3, None, "E_ARG"), (4, None, "E_ARG"), (5, None, "E_ARG"), (6, None, "E_ARG"),
     (7, -1, "E_ARG"), (8, 0, "E_ARG"), (9, 0, "E_ARG"), (10, -1, "E_ARG"), (10, 1 << 28, "E_LIMIT"),
-])
+] + [(i, P + 1, "E_ARG") for i in range(7)])
 def test_release_refuses(bmb, at, value, code):
     args = [P] * 7 + [4, 8, 16, 32, None]
     args[at] = value
@@ -80,6 +80,7 @@ def test_release_refuses(bmb, at, value, code):
     (dict(repetition=P), {}), (dict(frequency=P), {}), (dict(presence=P), {}), (dict(history=P, history_stride=4), {}),
     (dict(history=P, history_lens=P, history_stride=-1), {}), (dict(bias_ids=P, bias_lens=P), {}), (dict(bias=P, bias_lens=P), {}),
     (dict(bias_ids=P, bias=P), {}), (dict(bias_ids=P, bias=P, bias_lens=P, bias_stride=-1), {}), (dict(allowed=P, allowed_stride=3), {}),
+    (dict(history=P, history_lens=P + 2, history_stride=4), {}), (dict(allowed=P + 1, allowed_stride=4), {}), ({}, dict(out=P + 2)),
     ({}, dict(out=None)), ({}, dict(logits=None)), ({}, dict(n=-1)), ({}, dict(V=-1)), ({}, dict(stride=99)),
 ])
 def test_adjust_refuses(bmb, rules, more):
@@ -102,6 +103,28 @@ def test_workspace_is_stated(bmb):
 def test_struct_layouts(bmb):
     """The ctypes mirrors have the C structs' sizes: pointers and 64-bit strides first, then ints."""
     assert C.sizeof(bmb.KvCache) == 5 * 8 + 5 * 4 + 4 and C.sizeof(bmb.LogitRules) == 10 * 8 + 3 * 4 + 4
+
+
+def test_long_texts_are_refused(bmb):
+    for rules in (dict(history=P, history_lens=P, history_stride=(1 << 30) + 1), dict(bias_ids=P, bias=P, bias_lens=P, bias_stride=(1 << 30) + 1)):
+        assert bmb.lib().bmb_logits_adjust(P, P, 2, 100, 100, bmb.LogitRules(**rules), None) == bmb.E_LIMIT
+    assert bmb.lib().bmb_logits_adjust(P, P, 1 << 30, 5000, 5000, bmb.LogitRules(), None) == bmb.E_LIMIT
+    assert bmb.lib().bmb_paged_kv_write(cache(bmb, heads=1 << 26), P, P, 384, P, 4, None) == bmb.E_LIMIT
+
+
+def test_structs_of_tensors(bmb):
+    import torch
+    k = torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16)
+    c = bmb.KvCache.of(k, k.clone())
+    assert (c.page_stride, c.token_stride, c.head_stride, c.type, c.pages, c.page_size, c.heads, c.head_size) == (2048, 128, 64, bmb.TYPE_BF16, 3, 16, 2, 64)
+    t = k.transpose(1, 2)
+    c = bmb.KvCache.of(t, t)
+    assert (c.page_size, c.heads, c.token_stride, c.head_stride) == (2, 16, 64, 128)
+    for a, b in ((k, k.float()), (k, k[:2]), (k.double(), k.double()), (k[0], k[0]), (k.transpose(2, 3), k.transpose(2, 3)), (k, t.contiguous().transpose(1, 2))):
+        with pytest.raises(ValueError):
+            bmb.KvCache.of(a, b)
+    r = bmb.LogitRules.of(history=torch.zeros(2, 7, dtype=torch.int32), history_lens=torch.zeros(2, dtype=torch.int32), allowed=torch.zeros(2, 4, dtype=torch.int32))
+    assert (r.history_stride, r.bias_stride, r.allowed_stride) == (7, 0, 4) and r.bias is None
 
 
 def test_oracle_assign_by_hand():
