@@ -145,20 +145,34 @@ struct Place {
         next_head(s, lens);
         return 1;
     }
+    // (on the device a warp's lanes together: 32 requests without tokens are passed over at a time)
     __host__ __device__ void next_head(const Shape &s, const int *lens) {
         tile = 0;
         if (++vhead < s.vheads) return;
-        vhead = 0;
-        for (tiles = 0; tiles == 0 && ++request < s.n;) {
+        vhead = tiles = 0;
+#ifdef __CUDA_ARCH__
+        const int lane = threadIdx.x & 31;
+        for (++request; request < s.n; request += 32) {
+            const int its = lane < s.n - request ? s.length(lens[request + lane]) : 0;
+            const unsigned some = __ballot_sync(0xffffffffu, its > 0);
+            if (some) {
+                len = __shfl_sync(0xffffffffu, its, __ffs(some) - 1);
+                request += __ffs(some) - 1;
+                tiles = s.tiles(len);
+                return;
+            }
+        }
+#else
+        while (tiles == 0 && ++request < s.n) {
             len = s.length(lens[request]);
             tiles = s.tiles(len);
         }
+#endif
     }
-    // to the next tile; how many places on it is (1 or 2)
-    __host__ __device__ int next(const Shape &s, const int *lens) {
-        if (++tile < tiles) return 1;
-        next_head(s, lens);
-        return 2;
+    // places from this tile to the next, and the way there
+    __host__ __device__ int step() const { return tile + 1 < tiles ? 1 : 2; }
+    __host__ __device__ void next(const Shape &s, const int *lens) {
+        if (++tile >= tiles) next_head(s, lens);
     }
 };
 
@@ -419,7 +433,8 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(q + lane * 32));
                 }
             }
-            load_place += load.next(s, p.lens);
+            load_place += load.step();
+            if (load_place < end) load.next(s, p.lens);
         };
         // ---- the head at hand ----
         // pieces of its queries: 16-bit types [HS / 16][first piece, second] (+ third for bf16), fp32 [HS / 8][4]
@@ -532,7 +547,8 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
             for (int i = 0; i < PA_STAGES - 1; ++i)
                 if (ahead_place < end) {
                     look_up(ahead, rows[i]);
-                    ahead_place += ahead.next(s, p.lens);
+                    ahead_place += ahead.step();
+                    if (ahead_place < end) ahead.next(s, p.lens);
                 }
 #pragma unroll
             for (int i = 0; i < PA_STAGES - 1; ++i) {
@@ -693,9 +709,10 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
                     for (int k = 0; k < 2; ++k) o[2 * d + k] = add2(o[2 * d + k], add2(make_float2(c[k][0], c[k][1]), make_float2(c[k][2], c[k][3])));
                 }
             }
-            const bool ends = here.tile + 1 == here.tiles, last = at_place + (ends ? 2 : 1) >= end;
+            const bool ends = here.tile + 1 == here.tiles, last = at_place + here.step() >= end;
             if (ends || last) end_head(ends);
-            at_place += here.next(s, p.lens);
+            at_place += here.step();
+            if (!last) here.next(s, p.lens);
             if (ends && !last) {
                 // the queries staged with the tile that is next, which has to have come
                 if (p.staged) {
@@ -1017,7 +1034,7 @@ int bmb_paged_attention_schedule_check(const int *host_lens, int n, int heads, i
             ++done;
             if (here.request >= n || here.request != all.request || here.vhead != all.vhead || here.tile != all.tile || line.warp_of(place) != w)
                 return fail(BMB_E_ARG, "paged_attention_schedule_check: warp %d has another tile at %lld", w, place);
-            const bool ends = here.tile + 1 == here.tiles, last = place + (ends ? 2 : 1) >= end;
+            const bool ends = here.tile + 1 == here.tiles, last = place + here.step() >= end;
             if (ends || last) {
                 if (!(begins && ends) && ++parts > 2) return fail(BMB_E_ARG, "paged_attention_schedule_check: warp %d has %d parts", w, parts);
                 const int b = w / PA_WARPS, first_block = line.warp_of(place - here.tile) / PA_WARPS;
@@ -1029,7 +1046,8 @@ int bmb_paged_attention_schedule_check(const int *host_lens, int n, int heads, i
                 }
                 begins = true;
             }
-            place += here.next(s, host_lens);
+            place += here.step();
+            here.next(s, host_lens);
         }
     }
     if (done != tiles) return fail(BMB_E_ARG, "paged_attention_schedule_check: %lld of %lld tiles", done, tiles);

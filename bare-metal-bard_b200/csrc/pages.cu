@@ -169,10 +169,6 @@ __global__ void __launch_bounds__(THREADS) release_k(int *free_pages, int *free_
         int *mine_stashed = stashed + w * stash;
         auto read = [&](auto &&use) {
             int r = 0;
-            if (from < to)
-#pragma unroll
-                for (int step = THREADS / 2; step > 0; step >>= 1)
-                    if (end_of[r + step - 1] <= from) r += step;
             for (long long f = from + lane; f - lane < to; f += 32 * AHEAD) {
                 int page[AHEAD];
 #pragma unroll
@@ -180,7 +176,14 @@ __global__ void __launch_bounds__(THREADS) release_k(int *free_pages, int *free_
                     const long long e = f + 32 * k;
                     page[k] = -1;
                     if (e < to) {
-                        while (end_of[r] <= e) ++r;
+                        // the first request that ends behind e: one of the next, or far on
+                        for (int i = 0; i < 4 && end_of[r] <= e; ++i) ++r;
+                        if (end_of[r] <= e) {
+                            r = 0;
+#pragma unroll
+                            for (int step = THREADS / 2; step > 0; step >>= 1)
+                                if (end_of[r + step - 1] <= e) r += step;
+                        }
                         page[k] = tables[(size_t)(base + r) * max_pages + (e - (r > 0 ? end_of[r - 1] : 0))];
                     }
                 }

@@ -118,6 +118,9 @@ def test_release(bmb, cuda, n, page, longest, share, in_place):
 
 
 def test_release_corners(bmb, cuda):
+    ends = np.zeros(1500, np.int64)
+    ends[[0, 1, 700, 1023, 1024, 1499]] = 1                                                         # few among many
+    run_release(bmb, cuda, np.zeros(4600, np.int64), 11, np.arange(1500) % 49, np.arange(4500).reshape(1500, 3), ends, 16, 4600)
     t = np.array([[0, 1, 2], [3, 4, 5]])
     run_release(bmb, cuda, np.zeros(6, np.int64), 0, [], np.zeros((0, 3), np.int64), [], 16, 6)
     run_release(bmb, cuda, np.zeros(6, np.int64), 4, [48, 48], t, [1, 1], 16, 6)                    # no room for all of them
@@ -248,6 +251,8 @@ def test_attention_long_and_uneven(bmb, cuda, name):
     check_attention(bmb, cuda, name, "tokens", [40000, 3, 0, 1, 9000, 1], 8, 1, 128, 100)
     check_attention(bmb, cuda, name, "heads", [1 + 37 * (i % 29) for i in range(700)], 2, 2, 32, 16)
     check_attention(bmb, cuda, name, "heads", [20000] + [i % 3 for i in range(1100)], 2, 1, 32, 16)
+    check_attention(bmb, cuda, name, "heads", [0] * 700 + [60] + [0] * 1500 + [3, 3000, 0, 9] + [0] * 400, 4, 2, 64, 16)
+    check_attention(bmb, cuda, name, "heads", [5] + [0] * 31 + [3] + [0] * 32 + [2000] + [0] * 33 + [4] + [0] * 200, 1, 1, 128, 16)
 
 
 @pytest.mark.parametrize("name", TYPES)
