@@ -799,7 +799,8 @@ int trainer_build(bmb_trainer *t, const bmb_train_config &c, unsigned seed) {
         fill(P_WTE, 0.02f); fill(P_WPE, 0.02f); ones(P_LN1W);
         fill(P_QKVW, 0.02f); fill(P_APW, resid); ones(P_LN2W);
         fill(P_FCW, 0.02f); fill(P_FPW, resid); ones(P_LNFW);
-        BMB_CUDA(cudaMemcpy(t->params, h.data(), pb, cudaMemcpyHostToDevice));
+        BMB_CUDA(cudaMemcpyAsync(t->params, h.data(), pb, cudaMemcpyHostToDevice, t->st));      // (on that stream: see bmb_trainer_set_params)
+        BMB_CUDA(cudaStreamSynchronize(t->st));
     }
     {
         Scope sc(t);
@@ -907,8 +908,9 @@ int bmb_trainer_get_params(bmb_trainer *t, float *host_out) {
 int bmb_trainer_set_params(bmb_trainer *t, const float *host_in) {
     if (!t || !host_in) return fail(BMB_E_ARG, "trainer_set_params: null argument");
     Scope sc(t);
-    BMB_CUDA(cudaStreamSynchronize(t->st));
-    BMB_CUDA(cudaMemcpy(t->params, host_in, t->num_params * sizeof(float), cudaMemcpyHostToDevice));
+    // On the trainer's stream: a cudaMemcpy from pageable memory returns when its last part has been staged, not when it has arrived, and this stream
+    // does not wait for the default one, so the rounded copies could be made of what was there before.
+    BMB_CUDA(cudaMemcpyAsync(t->params, host_in, t->num_params * sizeof(float), cudaMemcpyHostToDevice, t->st));
     BMB_TRY(refresh_shadow(t));
     BMB_CUDA(cudaStreamSynchronize(t->st));
     return BMB_OK;
@@ -1228,7 +1230,7 @@ int bmb_trainer_load(bmb_trainer *t, const char *path, int load_optimizer_state,
     auto slurp = [&](float *dev, const char *what) {
         if (rc != BMB_OK) return;
         if (fread(buf.data(), sizeof(float), t->num_params, f) != t->num_params) { rc = fail(BMB_E_ARG, "%s: %s truncated", path, what); return; }
-        if (cudaMemcpy(dev, buf.data(), t->num_params * sizeof(float), cudaMemcpyHostToDevice) != cudaSuccess)
+        if (cudaMemcpyAsync(dev, buf.data(), t->num_params * sizeof(float), cudaMemcpyHostToDevice, t->st) != cudaSuccess || cudaStreamSynchronize(t->st) != cudaSuccess)
             rc = fail(BMB_E_CUDA, "trainer_load: copy of %s failed", what);
     };
     if (rc == BMB_OK) cudaStreamSynchronize(t->st);
