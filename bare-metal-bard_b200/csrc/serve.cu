@@ -50,7 +50,7 @@ struct Arena {
     ~Arena() { if (base) cudaFree(base); }
     template <typename T>
     T *take(size_t count) {
-        T *p = reinterpret_cast<T *>(base + used);
+        T *p = reinterpret_cast<T *>((uintptr_t)base + used);
         used += (count * sizeof(T) + 255) / 256 * 256;
         return p;
     }
@@ -60,7 +60,7 @@ constexpr int SV_PAGE = 16;
 
 struct Buffers {
     float *x, *y, *ln, *qkv, *att, *h, *g, *mean, *rstd, *lse, *last, *logits, *probs, *losses;
-    int *tokens, *positions, *slots, *packed_slots, *packed_positions, *starts, *lens, *lens_next, *grows, *done, *tables, *stack, *free_pages, *zeros, *history, *history_lens,
+    int *tokens, *positions, *slots, *packed_slots, *packed_positions, *starts, *lens, *grows, *done, *tables, *stack, *free_pages, *zeros, *history, *history_lens,
         *prompt_lens;
     float *repetition, *frequency, *presence;
     char *k, *v;
@@ -130,7 +130,11 @@ int generate_texts(const ServeModel &m, int n, const int *host_prompts, int prom
     };
     lay_out();                           // (how much it is)
     const size_t bytes = arena.used;
-    BMB_CUDA(cudaMalloc(&arena.base, bytes));
+    if (cudaMalloc(&arena.base, bytes) != cudaSuccess) {
+        arena.base = nullptr;
+        cudaGetLastError();              // (the next launch is not to find it)
+        return fail(BMB_E_CUDA, "trainer_generate_batch: no %zu bytes for %d texts of up to %d tokens", bytes, n, longest);
+    }
     arena.used = 0;
     lay_out();
     struct Idle {                        // the arena goes when nothing reads it any more

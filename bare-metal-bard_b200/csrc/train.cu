@@ -1371,8 +1371,8 @@ int bmb_trainer_generate(bmb_trainer *t, int start_token, int steps, unsigned se
 
 int bmb_trainer_generate_batch(bmb_trainer *t, int n, const int *host_prompts, int prompt_stride, const int *host_prompt_lens, int steps, unsigned seed,
                                const bmb_batch_sampling *how, int *host_tokens_out) {
-    if (!t || n < 0 || steps < 0 || !how || !(how->temperature > 0.0f) || !(how->repetition > 0.0f) || how->frequency != how->frequency ||
-        how->presence != how->presence || how->cache_type < BMB_TYPE_FP32 || how->cache_type > BMB_TYPE_FP16)
+    if (!t || n < 0 || steps < 0 || !how || !(how->temperature > 0.0f) || !(how->repetition > 0.0f) || !std::isfinite(how->temperature) ||
+        !std::isfinite(how->repetition) || !std::isfinite(how->frequency) || !std::isfinite(how->presence) || how->cache_type < BMB_TYPE_FP32 || how->cache_type > BMB_TYPE_FP16)
         return fail(BMB_E_ARG, "trainer_generate_batch: bad argument");
     if (n == 0 || steps == 0) return BMB_OK;
     if (!host_prompts || !host_prompt_lens || !host_tokens_out) return fail(BMB_E_ARG, "trainer_generate_batch: a null pointer");

@@ -131,7 +131,8 @@ def test_refusals(bmb, cuda):
     t = bmb.Trainer(seed=9, max_seq_len=32, vocab_size=65, padded_vocab=128, n_layer=1, n_head=2, n_embd=64, B=1, T=32, math=bmb.MATH_FP32)
     assert t.generate_batch([], 5, seed=1) == [] and t.generate_batch([[1]], 0, seed=1) == [[]]
     for prompts, steps, how in [([[1] * 20], 13, {}), ([[]], 3, {}), ([[65]], 3, {}), ([[-1]], 3, {}), ([[1]], 3, dict(temperature=0.0)), ([[1]], 3, dict(repetition=0.0)),
-                                ([[1]], 3, dict(frequency=float("nan"))), ([[1]], 3, dict(cache=3)), ([[1]], -1, {})]:
+                                ([[1]], 3, dict(frequency=float("nan"))),
+                                ([[1]], 3, dict(presence=float("inf"))), ([[1]], 3, dict(temperature=float("inf"))), ([[1]], 3, dict(cache=3)), ([[1]], -1, {})]:
         with pytest.raises(bmb.BmbError):
             t.generate_batch(prompts, steps, seed=1, **how)
     assert len(t.generate_batch([[1] * 20], 12, seed=1)[0]) == 12
