@@ -28,8 +28,8 @@ __global__ void __launch_bounds__(KW_THREADS) kv_write_k(const __grid_constant__
     let_successor_start();
     wait_for_predecessor();
     const long long at = (long long)blockIdx.x * KW_THREADS + threadIdx.x;
+    if (at >= (long long)tokens * units) return;              // (before the division: its result is an int)
     const int token = (int)div_near(at, units), e = (int)(at - (long long)token * units) * E;
-    if (token >= tokens) return;
     const int slot = slots[token];
     float x[2][E];
 #pragma unroll

@@ -538,3 +538,17 @@ def test_attention_with_blocks_for_each_head(bmb, cuda, name):
             check_attention(bmb, cuda, name, "heads", [max(L - 7 * i, 0) for i in range(24)], 12, 12, hs, 16, lse=False)
             check_attention(bmb, cuda, name, "interleaved", [L, 3, 0], 17, 1, hs, 24)
         check_attention(bmb, cuda, name, "tokens", [0, 5, 0], 9, 1, hs, 16)
+
+
+def test_write_of_as_many_rows_as_an_int_counts(bmb, cuda):
+    """2^31 - 1 rows, all but the first and the last left out: the threads behind the last row are beyond an int."""
+    torch = cuda
+    tokens = 2 ** 31 - 1
+    slots = torch.full((tokens,), -1, dtype=torch.int32, device="cuda")
+    slots[0], slots[-1] = 3, 17
+    k, v = (torch.zeros(2, 16, 1, 32, device="cuda") for _ in range(2))
+    row = torch.arange(64, dtype=torch.float32, device="cuda")
+    bmb.call("bmb_paged_kv_write", bmb.KvCache.of(k, v), row, row[32:], 0, slots, tokens, torch.cuda.current_stream().cuda_stream)
+    for got, want in ((k, row[:32]), (v, row[32:])):
+        rows = got.view(32, 32)
+        assert torch.equal(rows[[3, 17]], want.expand(2, 32)) and not rows[[i for i in range(32) if i not in (3, 17)]].any()
