@@ -1006,7 +1006,7 @@ size_t bmb_paged_attention_workspace(int heads, int kv_heads, int head_size) {
 
 int bmb_paged_attention_schedule_check(const int *host_lens, int n, int heads, int kv_heads, int head_size, int type, int max_len, int blocks,
                                        long long *tiles_out, int *joined_out) {
-    if (!host_lens || n <= 0 || kv_heads <= 0 || heads % kv_heads || max_len <= 0 || blocks <= 0 || type < BMB_TYPE_FP32 || type > BMB_TYPE_FP16 ||
+    if (!host_lens || n <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_len <= 0 || blocks <= 0 || blocks > PA_MOST_BLOCKS || type < BMB_TYPE_FP32 || type > BMB_TYPE_FP16 ||
         (head_size != 32 && head_size != 64 && head_size != 128))
         return fail(BMB_E_ARG, "paged_attention_schedule_check: bad argument");
     const Shape s = attend_shape(n, heads, kv_heads, head_size, type, max_len);

@@ -337,7 +337,7 @@ int bmb_paged_kv_write(const bmb_kv_cache *cache, const float *k, const float *v
  * streams, or two graphs that may run at once, have one each); its contents need no preparation and mean nothing afterwards.
  * Products and sums are of fp32 accuracy whatever the cache's type.  An infinity or NaN in q, or in a key or value that counts,
  * makes the outputs that it enters NaN. */
-/* bmb_paged_attention_schedule_check replays on the host how a call on `blocks` SMs divides its work (launches nothing, no GPU needed) and
+/* bmb_paged_attention_schedule_check replays on the host how a call of `blocks` thread blocks (at most 512) divides its work (launches nothing, no GPU needed) and
  * returns 0 when every tile of every head is worked on exactly once and every part is joined; *joined_out: heads whose parts lie
  * in several blocks.  max_len: max_pages * page_size. */
 int bmb_paged_attention_schedule_check(const int *host_lens, int n, int heads, int kv_heads, int head_size, int type, int max_len,

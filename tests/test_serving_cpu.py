@@ -163,3 +163,12 @@ def test_every_tile_is_worked_on_once(bmb, blocks, type_, hs):
             assert joined.value <= blocks
             most = max(most, joined.value)
     assert most > 0 or blocks == 1
+
+
+@pytest.mark.parametrize("at,value", [(0, None), (1, 0), (2, 0), (2, -2), (3, 0), (3, 4), (4, 96), (5, 3), (6, 0), (7, 0), (7, 513), (7, (1 << 31) - 1)])
+def test_schedule_check_refuses(bmb, at, value):
+    lens = (C.c_int * 2)(5, 300)
+    args = [C.addressof(lens), 2, 6, 2, 64, 0, 1000, 148, None, None]
+    assert bmb.lib().bmb_paged_attention_schedule_check(*args) == 0
+    args[at] = value
+    assert bmb.lib().bmb_paged_attention_schedule_check(*args) == bmb.E_ARG
