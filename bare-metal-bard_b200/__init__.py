@@ -73,11 +73,30 @@ class LogitRules(C.Structure):
 
     @classmethod
     def of(cls, **parts):
-        """The rules in tensors (each optional; history, bias_ids and allowed with a row for each text).  It keeps them alive."""
+        """The rules in tensors (each optional; history, bias_ids, bias and allowed with a row for each text, int32 and
+        float32 as in the C struct).  Rows may be the fronts of longer ones, which have to be there to their end: a call may
+        read whole rows.  It keeps them alive."""
+        rows = {"history": "history_stride", "bias_ids": "bias_stride", "bias": "bias_stride", "allowed": "allowed_stride"}
         r = cls(**{k: ptr(t) for k, t in parts.items()})
-        for name, stride in (("history", "history_stride"), ("bias_ids", "bias_stride"), ("allowed", "allowed_stride")):
-            if parts.get(name) is not None:
-                setattr(r, stride, parts[name].stride(0))
+        for name, t in parts.items():
+            if t is None:
+                continue
+            floats = name in ("repetition", "frequency", "presence", "bias")
+            if str(t.dtype) not in (("torch.float32",) if floats else ("torch.int32", "torch.uint32")):
+                raise ValueError(f"{name}: {t.dtype}")
+            if name not in rows:
+                if t.numel() > 1 and not t.is_contiguous():
+                    raise ValueError(f"{name}: its elements do not lie side by side")
+                continue
+            if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+                raise ValueError(f"{name}: a row for each text, its elements side by side")
+            stride = t.stride(0) if t.shape[0] > 1 and t.shape[1] > 0 else t.shape[1]
+            there = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+            if stride < t.shape[1] or t.shape[0] * stride > there:
+                raise ValueError(f"{name}: rows {stride} apart are not in the tensor's memory to their end")
+            if name == "bias" and parts.get("bias_ids") is not None and stride != r.bias_stride:
+                raise ValueError("bias: its rows lie as those of bias_ids do")
+            setattr(r, rows[name], stride)
         r.tensors = parts
         return r
 

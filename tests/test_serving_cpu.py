@@ -165,6 +165,24 @@ def test_every_tile_is_worked_on_once(bmb, blocks, type_, hs):
     assert most > 0 or blocks == 1
 
 
+def test_rules_of_tensors_that_do_not_hold_their_rows(bmb):
+    """A call may read rows to their end, whatever the lengths are: the fronts of rows are taken, their backs, whose last one ends
+    outside the memory, are not, nor are rows that lie on one another, other types and elements that lie apart."""
+    import torch
+    i, f = torch.zeros(3, 20, dtype=torch.int32), torch.zeros(3, 20)
+    one = dict(history_lens=torch.zeros(3, dtype=torch.int32))
+    assert bmb.LogitRules.of(history=i[:, :7], **one).history_stride == 20
+    assert bmb.LogitRules.of(history=i[:2, 13:], **one).history_stride == 20
+    assert bmb.LogitRules.of(history=i[2:, 13:], **one).history_stride == 7
+    assert bmb.LogitRules.of(history=torch.zeros(3, 0, dtype=torch.int32), **one).history_stride == 0
+    assert bmb.LogitRules.of(bias_ids=i[:, :5], bias=f[:, 2:7][:2], bias_lens=one["history_lens"]).bias_stride == 20
+    for bad in (dict(history=i[:, 1:]), dict(history=i[:1].expand(3, 20)), dict(history=i.t()), dict(history=i[0]), dict(history=i.long()), dict(allowed=i[:, 19:]),
+                dict(allowed=f), dict(bias_ids=i, bias=torch.zeros(3, 5)), dict(bias=f.double()), dict(bias=f[:, 3:]), dict(repetition=f[:, 0]),
+                dict(frequency=i[0]), dict(presence=f[0].half()), dict(history_lens=i[:, 0]), dict(prompt_lens=torch.zeros(3, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            bmb.LogitRules.of(**bad)
+
+
 @pytest.mark.parametrize("at,value", [(0, None), (1, 0), (2, 0), (2, -2), (3, 0), (3, 4), (4, 96), (5, 3), (6, 0), (7, 0), (7, 513), (7, (1 << 31) - 1)])
 def test_schedule_check_refuses(bmb, at, value):
     lens = (C.c_int * 2)(5, 300)
