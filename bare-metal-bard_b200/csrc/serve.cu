@@ -137,18 +137,17 @@ int generate_texts(const ServeModel &m, int n, const int *host_prompts, int prom
     }
     arena.used = 0;
     lay_out();
-    struct Idle {                        // the arena goes when nothing reads it any more
-        cudaStream_t st;
-        ~Idle() { cudaStreamSynchronize(st); }
-    } idle{m.st};
-
     cudaStream_t st = m.st;
     auto upload = [&](void *dst, const void *src, size_t size) -> int {
-        BMB_CUDA(cudaMemcpyAsync(dst, src, size, cudaMemcpyHostToDevice, st));      // (from pageable memory: read before it returns)
+        BMB_CUDA(cudaMemcpyAsync(dst, src, size, cudaMemcpyHostToDevice, st));      // (nothing that it reads changes before the next synchronise)
         return BMB_OK;
     };
     std::vector<int> tokens(rows, 0), history((size_t)n * longest, 0), ids(pages), ones(n, 1), none(n, 0), last(n), ended(n, 0);
-    std::vector<float> same(n);
+    std::vector<float> same(3 * (size_t)n), probs((size_t)n * Vp);
+    struct Idle {                        // arena and vectors go when nothing reads or writes them any more
+        cudaStream_t st;
+        ~Idle() { cudaStreamSynchronize(st); }
+    } idle{m.st};
     std::iota(ids.begin(), ids.end(), 0);
     for (int i = 0; i < n; ++i) {
         std::copy_n(host_prompts + (size_t)i * prompt_stride, host_prompt_lens[i], tokens.begin() + i * width);
@@ -165,8 +164,8 @@ int generate_texts(const ServeModel &m, int n, const int *host_prompts, int prom
     const float penalties[] = {how.repetition, how.frequency, how.presence};
     float *of_rows[] = {b.repetition, b.frequency, b.presence};
     for (int j = 0; j < 3; ++j) {
-        std::fill(same.begin(), same.end(), penalties[j]);
-        BMB_TRY(upload(of_rows[j], same.data(), n * sizeof(float)));
+        std::fill_n(same.begin() + (size_t)j * n, n, penalties[j]);
+        BMB_TRY(upload(of_rows[j], same.data() + (size_t)j * n, n * sizeof(float)));
     }
     BMB_CUDA(cudaMemsetAsync(b.lens, 0, n * sizeof(int), st));
     BMB_CUDA(cudaMemsetAsync(b.zeros, 0, n * sizeof(int), st));
@@ -221,7 +220,6 @@ int generate_texts(const ServeModel &m, int n, const int *host_prompts, int prom
         return product(n, Vp, C, columns > 1 ? b.last : b.ln, m.wte_w, nullptr, b.logits);
     };
 
-    std::vector<float> probs((size_t)n * Vp);
     std::vector<std::mt19937> rng;
     for (int i = 0; i < n; ++i) rng.emplace_back(seed + i);
     std::uniform_real_distribution<float> uni(0.0f, 1.0f);
