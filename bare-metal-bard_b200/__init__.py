@@ -260,7 +260,11 @@ def _arg(a):
 
 def call(name, *args):
     """Call a status-returning entry point with tensors turned into pointers."""
-    status = getattr(_lib or lib(), name)(*[a if a.__class__ in _PLAIN else _arg(a) for a in args])
+    try:                                  # (most have tensors alone: asking each of 11 what it is took 0.5 us of a call's 6.1)
+        plain = [a if a.__class__ in _PLAIN else a.data_ptr() for a in args]
+    except AttributeError:
+        plain = [a if a.__class__ in _PLAIN else _arg(a) for a in args]
+    status = getattr(_lib or lib(), name)(*plain)
     if status:
         check(status, name)
 
