@@ -102,7 +102,9 @@ __global__ void __launch_bounds__(THREADS) assign_k(int *tables, int *lens_out, 
             lens_out[i] = served ? L + A : L;
             if (starts) starts[i] = begin_of[threadIdx.x];
         }
-        for (int t = chunk_begin + me * THREADS + (int)threadIdx.x; t < chunk_end; t += BLOCKS * THREADS) {
+        // (counted in 64 bits: the last step may end behind an int)
+        for (long long next = (long long)chunk_begin + me * THREADS + threadIdx.x; next < chunk_end; next += BLOCKS * THREADS) {
+            const int t = (int)next;
             int r = 0;                                        // the last request that begins at t or before it
 #pragma unroll
             for (int step = THREADS / 2; step > 0; step >>= 1)
