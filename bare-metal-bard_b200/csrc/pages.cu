@@ -238,6 +238,7 @@ constexpr int PG_FEW_REQUESTS = 256, PG_FEW = 1024, PG_SOME_TOKENS = 2048, PG_SO
 int check_pool(const char *what, int n, int max_pages, int page_size, int pages) {
     if (n < 0 || max_pages <= 0 || page_size <= 0 || pages < 0)
         return fail(BMB_E_ARG, "%s: bad sizes (n=%d max_pages=%d page_size=%d pages=%d)", what, n, max_pages, page_size, pages);
+    if (n > INT_MAX - (PG_MOST - 1)) return fail(BMB_E_LIMIT, "%s: %d requests", what, n);      // (the first one behind the last stretch is an int)
     if ((long long)pages * page_size > INT_MAX || (long long)max_pages * page_size > INT_MAX)
         return fail(BMB_E_LIMIT, "%s: %d (a row of the tables: %d) pages of %d tokens are beyond an int", what, pages, max_pages, page_size);
     return BMB_OK;

@@ -311,7 +311,8 @@ typedef struct bmb_kv_cache {
  *   positions  [max_tokens] a token's index in its request, owners [max_tokens] the request (each may be NULL)
  *   starts     [n + 1] where each request's tokens begin and the last one's end, at most max_tokens (may be NULL)
  *   free_left  pages left on the stack (may be free_count itself); free_pages is not written
- * All pointers are device pointers, lens and new_lens included; sums of lengths are 64-bit. */
+ * All pointers are device pointers, lens and new_lens included; sums of lengths are 64-bit.  Here and in bmb_pages_release n is at most 2^31 - 1024
+ * and a pool's tokens and those of a row of the tables fit an int (BMB_E_LIMIT). */
 int bmb_pages_assign(int *tables, int *lens_out, int *slots, int *positions, int *owners, int *starts, int *free_left,
                      const int *lens, const int *new_lens, const int *free_pages, const int *free_count, int n, int max_pages,
                      int page_size, int pages, int max_tokens, void *stream);

@@ -190,3 +190,10 @@ def test_schedule_check_refuses(bmb, at, value):
     assert bmb.lib().bmb_paged_attention_schedule_check(*args) == 0
     args[at] = value
     assert bmb.lib().bmb_paged_attention_schedule_check(*args) == bmb.E_ARG
+
+
+@pytest.mark.parametrize("n", [(1 << 31) - 1023, (1 << 31) - 1])
+def test_more_requests_than_stretches_can_count_are_refused(bmb, n):
+    """Requests are taken in stretches of up to 1024, the first one behind the last of which is an int too."""
+    assert bmb.lib().bmb_pages_assign(*[P] * 11, n, 8, 16, 32, 64, None) == bmb.E_LIMIT
+    assert bmb.lib().bmb_pages_release(*[P] * 7, n, 8, 16, 32, None) == bmb.E_LIMIT
