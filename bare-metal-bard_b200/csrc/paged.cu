@@ -847,12 +847,12 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
         }
         cluster_sync();                                       // (the others have read this block's part)
     }
-    // ---- requests without tokens ----
-    for (int r = blockIdx.x; r < s.n; r += gridDim.x) {
-        if (s.length(r == (int)blockIdx.x ? len_here : p.lens[r]) > 0) continue;
-        for (int i = threadIdx.x; i < s.heads * HS; i += PA_THREADS) p.out[r * p.out_stride + i] = 0.0f;
+    // ---- requests without tokens ----  (a row, and what is behind the last request or head, may be beyond an int)
+    for (long long r = blockIdx.x; r < s.n; r += gridDim.x) {
+        if (s.length(r == blockIdx.x ? len_here : p.lens[r]) > 0) continue;
+        for (long long i = threadIdx.x; i < (long long)s.heads * HS; i += PA_THREADS) p.out[r * p.out_stride + i] = 0.0f;
         if (p.lse)
-            for (int h = threadIdx.x; h < s.heads; h += PA_THREADS) p.lse[(size_t)r * s.heads + h] = -INFINITY;
+            for (long long h = threadIdx.x; h < s.heads; h += PA_THREADS) p.lse[r * s.heads + h] = -INFINITY;
     }
 }
 

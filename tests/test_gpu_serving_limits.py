@@ -28,3 +28,20 @@ def test_assign_of_as_many_tokens_as_an_int_counts(bmb, cuda, before):
         assert torch.equal(positions[at:to], torch.arange(at - 5, to - 5, dtype=torch.int32, device="cuda"))
     assert [int(x[T]) for x in (slots, positions, owners)] == [77] * 3
     assert starts.tolist() == [0, 5] + [T] * (n - 1) and lens.tolist() == [5] + [0] * (n - 1) and int(free) == 3
+
+
+def test_attention_of_rows_that_are_longer_than_an_int_counts(bmb, cuda):
+    """2^25 heads of 64: a row of outputs has 2^31 elements, and all of them are written, of a request without tokens too."""
+    torch = cuda
+    heads, hs = 1 << 25, 64
+    k, v = (torch.randn(1, 16, 1, hs, device="cuda").bfloat16() for _ in range(2))
+    q = torch.ones(heads * hs, device="cuda")
+    out, lse = torch.full((2, heads * hs), 77.0, device="cuda"), torch.full((2, heads), 77.0, device="cuda")
+    ws = torch.empty(bmb.paged_attention_workspace(heads, 1, hs), dtype=torch.uint8, device="cuda")
+    bmb.call("bmb_paged_attention", out, lse, q, bmb.KvCache.of(k, v), i32(torch, [[0], [0]]), i32(torch, [0, 1]), 2, heads, 0, heads * hs, 1, 0.0, ws, ws.numel(),
+             torch.cuda.current_stream().cuda_stream)
+    for part in out[0].split(1 << 28):
+        assert (part == 0).all()
+    for part in out[1].view(heads, hs).split(1 << 22):
+        assert (part == v[0, 0].float()).all()               # (one token: its weight is 1, and a bf16 value's product with that is exact)
+    assert (lse[0] == -float("inf")).all() and (lse[1] == 0).all()
