@@ -741,8 +741,8 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
         for (int i = 0; i < 2 * PA_WARPS; ++i)
             if (same(of, entry(i))) top = fmaxf(top, part_m[i >> 1][i & 1][r]);
         const float l = part_l[e >> 1][e & 1][r];
-        // (NaN where the sum is: its maximum may be that of nothing)
-        weight[e][r] = !of.w || l == 0.0f ? 0.0f : l == l ? exp2f(part_m[e >> 1][e & 1][r] - top) : l;
+        // (below 0: there is none.  NaN where the sum is: its maximum may be that of nothing)
+        weight[e][r] = !of.w ? -1.0f : l == 0.0f ? 0.0f : l == l ? exp2f(part_m[e >> 1][e & 1][r] - top) : l;
     } else if (w == PA_WARPS - 1) {
         const int4 of = lane < 2 * PA_WARPS ? entry(lane) : make_int4(0, 0, 0, 0);
         bool first = of.w;
@@ -763,9 +763,9 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
     // (of a cluster: the block's part of the head, in the second place of the first warp's ring)
     float *block_o = reinterpret_cast<float *>(smem + 2 * PA_TILE), *block_m = block_o + PA_ROWS * HS, *block_l = block_m + PA_ROWS;
     static_assert(PA_ROWS * (HS + 2) * sizeof(float) <= 2 * PA_TILE, "");
-    if (p.alone > 1 && threadIdx.x < PA_ROWS) {               // (nothing, if it has no tile)
+    if (p.alone > 1 && threadIdx.x < PA_ROWS) {               // (none, if it has no tile)
         block_m[threadIdx.x] = -INFINITY;
-        block_l[threadIdx.x] = 0.0f;
+        block_l[threadIdx.x] = -1.0f;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < groups * rows_kept * (HS / 4); i += PA_THREADS) {
@@ -777,11 +777,11 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
         float all = 0.0f, top = -INFINITY, x[4] = {};
 #pragma unroll
         for (int k = 0; k < 2 * PA_WARPS; ++k) {
-            const float by = k < e0 || k > e1 ? 0.0f : weight[k][r];      // (0 also for an entry between them that is none)
+            const float by = k < e0 || k > e1 ? -1.0f : weight[k][r];     // (below 0 also for an entry between them that is none)
             const float4 v = *reinterpret_cast<const float4 *>(
                 (k & 1 ? smem + (k >> 1) * (PA_STAGES * 2 * PA_TILE) : smem + PA_WARPS * PA_STAGES * 2 * PA_TILE + (k >> 1) * rows_kept * HS * sizeof(float)) +
                 (r * HS + d) * sizeof(float));
-            const bool use = by != 0.0f;
+            const bool use = !(by < 0.0f);                    // (a weight of 0 is one: 0 times an infinity or NaN is NaN)
             all = use ? fmaf(part_l[k >> 1][k & 1][r], by, all) : all;
             top = use ? fmaxf(top, part_m[k >> 1][k & 1][r]) : top;
             x[0] = use ? fmaf(v.x, by, x[0]) : x[0];
@@ -822,7 +822,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
 #pragma unroll
             for (int k = 0; k < PA_CLUSTER; ++k) {
                 m[k] = -INFINITY;
-                l[k] = 0.0f;
+                l[k] = -1.0f;
                 if (k >= p.alone) continue;
                 m[k] = read_of<float>(block_m + r, k);
                 l[k] = read_of<float>(block_l + r, k);
@@ -831,8 +831,8 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
             }
 #pragma unroll
             for (int k = 0; k < PA_CLUSTER; ++k) {
-                if (l[k] == 0.0f) continue;
-                const float by = l[k] == l[k] ? exp2f(m[k] - top) : l[k];
+                if (l[k] < 0.0f) continue;
+                const float by = l[k] == 0.0f ? 0.0f : l[k] == l[k] ? exp2f(m[k] - top) : l[k];
                 all = fmaf(l[k], by, all);
                 x[0] = fmaf(v[k].x, by, x[0]);
                 x[1] = fmaf(v[k].y, by, x[1]);

@@ -45,3 +45,99 @@ def test_attention_of_rows_that_are_longer_than_an_int_counts(bmb, cuda):
     for part in out[1].view(heads, hs).split(1 << 22):
         assert (part == v[0, 0].float()).all()               # (one token: its weight is 1, and a bf16 value's product with that is exact)
     assert (lse[0] == -float("inf")).all() and (lse[1] == 0).all()
+
+
+# ---- infinities, NaN, the largest numbers -------------------------------------------------------------------------------
+
+def formula(torch, q, k, v, lens, scale):
+    """Softmax attention of q [n, heads, hs] over k and v [n, longest, kv, hs] in 64 bits, with what IEEE makes of infinities and NaN, a score
+    of -infinity having weight 0; and how far fp32 may be from it where it is finite.  As serving_oracle.attention_bounds has it (errors of a score
+    d; of a weight twice that), but for each column by itself and with two roundings for each token in the sums, which are one chain
+    where a sum is not finite or an element is near the largest.  Of an fp16 cache the rest of an element of q behind its first piece is a half too, in
+    units in which the row's largest is 2^14 at least: off by 2^-25 (half the smallest half) at most, 2^-39 of the row's largest, besides what is counted above."""
+    n, heads, hs = q.shape
+    group, u = heads // k.shape[2], 2.0 ** -24
+    out, bound = torch.zeros(2, n, heads, hs, dtype=torch.float64, device=q.device)
+    lse, lse_bound = torch.full((n, heads), -float("inf"), dtype=torch.float64, device=q.device), torch.zeros(n, heads, dtype=torch.float64, device=q.device)
+    for i in range(n):
+        for h in range(heads):
+            x, y = k[i, :lens[i], h // group].double(), v[i, :lens[i], h // group].double()
+            terms = x * q[i, h].double()
+            s = terms.sum(1) * scale
+            if torch.isnan(s).any() or (s == float("inf")).any():
+                out[i, h] = lse[i, h] = float("nan")
+                continue
+            some = s > -float("inf")
+            if not some.any():
+                continue
+            top = s.max()
+            w = torch.exp(s - top)
+            out[i, h] = (w[:, None] * y).sum(0) / w.sum()
+            lse[i, h] = top + torch.log(w.sum())
+            d = (hs / 4 + 8) * u * (terms[some].abs().sum(1) * abs(scale)).max()
+            if k.dtype == torch.float16:
+                d = d + 2.0 ** -39 * q[i, h].double().abs().max() * (x[some].abs().sum(1) * abs(scale)).max()
+            rest = (2 * lens[i] + 64) * u
+            bound[i, h] = (2 * d + rest) * torch.where(torch.isfinite(y), y, 0.0).abs().amax(0)
+            lse_bound[i, h] = d + rest + 2 * u * lse[i, h].abs()
+    return out, bound, lse, lse_bound
+
+
+def check_limits(bmb, torch, q, k, v, lens, scale, width, loose=None):
+    """Against the formula; `width`: pages of a row of the tables, by which attention is divided.  loose: (request, head, column) where NaN and
+    an infinity are alike, a weight being 0 in fp32 that is not in 64 bits."""
+    n, heads, hs = q.shape
+    longest, kv = k.shape[1:3]
+    page = 16
+    each = -(-longest // page)
+    ids = torch.randperm(n * each)
+    tables = torch.full((n, width), -1, dtype=torch.int32)
+    tables[:, :each] = ids.view(n, each)
+    pools = []
+    for x in (k, v):
+        pool = torch.full((n * each, page, kv, hs), float("nan"), dtype=x.dtype, device="cuda")
+        rows = torch.nn.functional.pad(x, (0, 0, 0, 0, 0, each * page - longest)).view(n * each, page, kv, hs)
+        pool[ids.cuda()] = rows
+        pools.append(pool)
+    out, lse = torch.full((n, heads, hs), 77.0, device="cuda"), torch.full((n, heads), 77.0, device="cuda")
+    ws = torch.empty(bmb.paged_attention_workspace(heads, kv, hs), dtype=torch.uint8, device="cuda")
+    bmb.call("bmb_paged_attention", out, lse, q, bmb.KvCache.of(*pools), tables.cuda(), i32(torch, lens), n, heads, heads * hs, heads * hs, width, scale, ws,
+             ws.numel(), torch.cuda.current_stream().cuda_stream)
+    want, bound, want_lse, lse_bound = formula(torch, q, k, v, lens, scale)
+    for got, want, bound in ((out.double(), want, bound), (lse.double(), want_lse, lse_bound)):
+        finite = torch.isfinite(want)
+        same = torch.where(finite, (got - want).abs() <= bound, (got == want) | (torch.isnan(got) & torch.isnan(want)))
+        if loose is not None and got.dim() == 3:
+            same[loose] = ~torch.isfinite(got[loose])
+        assert same.all(), (torch.argwhere(~same)[:4].tolist(), got[~same][:4].tolist(), want[~same][:4].tolist(), bound[~same][:4].tolist())
+    return out
+
+
+def texts(torch, name, n, longest, heads, kv, hs, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *shape: torch.randn(*shape, generator=g, device="cuda")
+    dt = dtype_of(torch, name)
+    return r(n, heads, hs), r(n, longest, kv, hs).to(dt), r(n, longest, kv, hs).to(dt)
+
+
+# heads, kv heads, head size, longest text, pages of a table's row: a cluster for each head; one block; the line, its heads in one
+# warp, in several of a block, over blocks
+FORMS = [(6, 2, 64, 40, 4), (2, 1, 32, 700, 44), (3, 3, 128, 300, 20), (18, 1, 64, 150, 10), (12, 12, 32, 33, 3000), (18, 1, 64, 300, 3000), (2, 1, 128, 6000, 3000),
+         (1, 1, 128, 20000, 3000)]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("heads,kv,hs,longest,width", FORMS)
+def test_a_value_that_is_not_finite_is_seen_however_small_its_weight(bmb, cuda, name, heads, kv, hs, longest, width):
+    """One token takes all and the other tokens' weights are 0 in fp32, those of whole parts of the text together; 0 times NaN is NaN."""
+    torch = cuda
+    for at in (0, longest // 3, longest - 2):
+        q, k, v = texts(torch, name, 2, longest, heads, kv, hs)
+        k[:, :, :, 0] = 0
+        k[:, longest // 2, :, 0] = 30
+        q[:, :, 0] = 30
+        v[0, at, 0, 5], v[0, at + 1, kv - 1, 9], v[1, at, kv - 1, 3] = float("nan"), float("inf"), -float("inf")
+        group = heads // kv
+        loose = torch.zeros(2, heads, hs, dtype=torch.bool, device="cuda")
+        loose[0, :group, 5] = loose[0, -group:, 9] = loose[1, -group:, 3] = True
+        check_limits(bmb, torch, q, k, v, [longest, longest - 1], 1.0, width, loose)
