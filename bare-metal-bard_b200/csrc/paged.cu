@@ -83,6 +83,12 @@ int run_write(const bmb_kv_cache &c, const float *k, const float *v, long long r
 // 4.5e-7 in the 2-norm for 2.8e-7).  Sums over tiles are kept in fp32 registers.  Masked and absent tokens are zeros in
 // shared memory with a weight of zero, whatever the memory there holds.
 //
+// Pieces of an infinity, and of an fp32 element within 2^-12 of the largest number, whose first piece is rounded to one, cancel to NaN where the formula
+// has an infinity or a finite result.  A score of NaN, and an infinity or NaN in a sum of values, is still there when a head ends; what lost its sign would
+// be NaN too, so sums that are finite are right.  A warp that had others works on those heads (its parts of them) once more when its run is
+// done, a token at a time in plain fp32: what it leaves is what the formula gives.  The check at a head's end and the code for it cost
+// 0.1 us of the 6.2 of one text of 256 tokens, 0.15 of 15.3 where heads end with nearly every tile, and nothing that can be told of 99.
+//
 // Bound by, and measured (us, caches cold): 609 MB of fp16, 8 requests of up to 32768 tokens, 32 heads on 8 of 128: 100, 6.1 TB/s, the loads.  203 MB of
 // fp32, 37 of up to 2777, 16 heads on 4 of 128: 44.5, and 101 MB of bf16, 64 of up to 1024, 12 heads of 64: 26.8: the loads alone take 40.8 and
 // 24.6 of that, at 6.2 TB/s behind 4 us before the first tile is there and in front of 4 for the last warps and the joins; the arithmetic alone 43.3
@@ -91,6 +97,7 @@ constexpr int PA_WARPS = 4, PA_THREADS = 32 * PA_WARPS, PA_STAGES = 3, PA_TILE =
 constexpr int PA_BLOCKS = 2, PA_MOST_BLOCKS = 512;          // blocks an SM, and in all
 constexpr size_t PA_SMEM = 112 * 1024;                       // dynamic shared memory with which two blocks fit an SM
 constexpr int PA_CLUSTER = 8;
+constexpr float LOWEST = -3.402823466e38f;                   // number of fp32
 
 // Blocks for each head, a cluster of them, or 0 for the line (below).  Where heads are few or short a cluster takes each alone: no line to find a
 // place in and no second launch, which together are 2 to 4 us of GPU time and 4 of the host's.  But then the longest head alone says how long it
@@ -323,14 +330,18 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
     Line line(0, 1);
     long long begin = 0;                                      // of this warp's run in the line, and its places, from 0: the next one and the end
     int at_place = 0, end = 0;
-    if (p.alone) {
+    // A warp's share of a head that a cluster has alone: to its first tile; how many there are.
+    auto share_alone = [&](Place &x) {
         const int head = blockIdx.x / p.alone, warp = (blockIdx.x - head * p.alone) * PA_WARPS + w, warps = p.alone * PA_WARPS;
-        here.request = head / s.vheads;
-        here.vhead = head - here.request * s.vheads;
-        here.len = s.length(p.lens[here.request]);
-        here.tiles = s.tiles(here.len);
-        here.tile = here.tiles * warp / warps;                // (few of them)
-        end = here.tiles * (warp + 1) / warps - here.tile;
+        x.request = head / s.vheads;
+        x.vhead = head - x.request * s.vheads;
+        x.len = s.length(p.lens[x.request]);
+        x.tiles = s.tiles(x.len);
+        x.tile = x.tiles * warp / warps;                      // (few of them)
+        return x.tiles * (warp + 1) / warps - x.tile;
+    };
+    if (p.alone) {
+        end = share_alone(here);
         __syncthreads();
     } else {
         // how many places (of one head each) lie before each thread's stretch of requests
@@ -444,6 +455,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
         float m = 0.0f, l = 0.0f, f = 0.0f;     // m in units of the scores as the products give them, f: log2's of one of those
         bool begins = false;
         int done = 0;                                         // parts kept for joining
+        bool again = false;                                   // there are heads whose sums are not finite (NaN in their first row's output or sum says which)
         // (x: a lane's elements of q, read ahead of what else waits for memory)
         auto read_queries = [&](const float *q, float (&x)[HS / 4]) {
             const int kept = min(PA_ROWS, s.group - (here.vhead % s.parts) * PA_ROWS);
@@ -501,6 +513,14 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
             const float top = m * f;                          // (-inf where nothing counted; f may be 0)
             const int kept = min(PA_ROWS, s.group - (here.vhead % s.parts) * PA_ROWS);
             l *= down;
+            float2 all[4] = {make_float2(l, l == 0.0f ? 0.0f : top), o[0], o[1], o[2]};
+#pragma unroll
+            for (int i = 3; i < HS / 8; ++i) all[i % 4] = add2(all[i % 4], o[i]);
+            all[0] = add2(add2(all[0], all[1]), add2(all[2], all[3]));
+            if (__any_sync(0xffffffffu, g < kept && !(fabsf(all[0].x + all[0].y) < INFINITY))) {
+                l = __int_as_float(0x7fffffff);               // NaN
+                again = true;
+            }
             if (begins && ends && p.alone <= 1) {
                 if (g >= kept) return;
                 const int h = (here.vhead / s.parts) * s.group + (here.vhead % s.parts) * PA_ROWS + g;
@@ -725,6 +745,65 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
                 begin_head(x);
             }
         }
+
+        // ---- heads whose sums are not finite, once more and without pieces ----
+        if (again) {
+            __syncwarp();
+            Place x;
+            int at = 0, part = 0;
+            if (p.alone) share_alone(x);
+            else at = x.set(s, p.lens, run_begin[w].request, run_begin[w].in);
+            while (at < end) {
+                const int t0 = x.tile, t1 = min(x.tiles, t0 + (end - at));
+                const bool whole = t0 == 0 && t1 == x.tiles && p.alone <= 1;
+                const int kept = min(PA_ROWS, s.group - (x.vhead % s.parts) * PA_ROWS), h0 = (x.vhead / s.parts) * s.group + (x.vhead % s.parts) * PA_ROWS;
+                float *to = whole ? p.out + x.request * p.out_stride + (long long)h0 * HS : part == 0 ? first_part : reinterpret_cast<float *>(ring);
+                const float found = whole ? to[0] : part_l[w][part][0];
+                if (found != found) {
+                    const int *table = p.tables + (size_t)x.request * p.max_pages;
+                    const int first = t0 * KEYS, behind = (int)min((long long)t1 * KEYS, (long long)x.len);
+                    for (int r = 0; r < kept; ++r) {
+                        float xq[HS / 32], y[HS / 32] = {}, top = -INFINITY, sum = 0.0f;      // columns lane, lane + 32, ...
+#pragma unroll
+                        for (int i = 0; i < HS / 32; ++i) xq[i] = queries(x)[r * HS + lane + 32 * i];
+#pragma unroll 1
+                        for (int key = first; key < behind; ++key) {
+                            const unsigned k = p.page_size.quotient(key);
+                            const int page = table[k];
+                            if ((unsigned)page >= (unsigned)p.c.pages) continue;
+                            const long long off = page * p.c.page_stride + (int)(key - k * p.page_size.by) * p.c.token_stride + (x.vhead / s.parts) * p.c.head_stride + lane;
+                            float score = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < HS / 32; ++i) score = fmaf(xq[i], (float)((const T *)p.c.k)[off + 32 * i], score);
+                            score = warp_sum(score) * p.scale * 1.4426950408889634f;
+                            const float mn = fmaxf(top, score), by = top == -INFINITY ? 0.0f : exp2f(top - mn);
+                            const float weigh = score == -INFINITY ? 0.0f : exp2f(score - mn);
+                            sum = fmaf(sum, by, weigh);
+#pragma unroll
+                            for (int i = 0; i < HS / 32; ++i) y[i] = fmaf(weigh, (float)((const T *)p.c.v)[off + 32 * i], y[i] * by);
+                            top = mn;
+                        }
+                        const float over = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+                        for (int i = 0; i < HS / 32; ++i) to[r * HS + lane + 32 * i] = y[i] * over;
+                        if (lane == 0) {
+                            if (!whole) {
+                                part_m[w][part][r] = sum == 0.0f ? -INFINITY : top;
+                                part_l[w][part][r] = sum;
+                            } else if (p.lse) {
+                                p.lse[(size_t)x.request * s.heads + h0 + r] = sum == 0.0f ? -INFINITY : fmaf(top, 0.6931471805599453f, logf(sum));
+                            }
+                        }
+                    }
+                }
+                part += !whole;
+                at += t1 - t0 + 1;
+                if (at < end) {
+                    x.tile = x.tiles - 1;
+                    x.next(s, p.lens);
+                }
+            }
+        }
     }
 
     // ---- heads that several of the block's warps, or blocks, have parts of ----
@@ -736,13 +815,11 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
     if (threadIdx.x < 2 * PA_WARPS * PA_ROWS) {
         const int e = threadIdx.x / PA_ROWS, r = threadIdx.x % PA_ROWS;
         const int4 of = entry(e);
-        float top = -INFINITY;
+        float top = LOWEST;                                   // (so that the weight of a maximum of -infinity is 0)
 #pragma unroll
         for (int i = 0; i < 2 * PA_WARPS; ++i)
             if (same(of, entry(i))) top = fmaxf(top, part_m[i >> 1][i & 1][r]);
-        const float l = part_l[e >> 1][e & 1][r];
-        // (below 0: there is none.  NaN where the sum is: its maximum may be that of nothing)
-        weight[e][r] = !of.w ? -1.0f : l == 0.0f ? 0.0f : l == l ? exp2f(part_m[e >> 1][e & 1][r] - top) : l;
+        weight[e][r] = of.w ? exp2f(part_m[e >> 1][e & 1][r] - top) : -1.0f;      // (below 0: there is none)
     } else if (w == PA_WARPS - 1) {
         const int4 of = lane < 2 * PA_WARPS ? entry(lane) : make_int4(0, 0, 0, 0);
         bool first = of.w;
@@ -817,7 +894,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
         const int kept = min(PA_ROWS, s.group - (vhead % s.parts) * PA_ROWS), h0 = (vhead / s.parts) * s.group + (vhead % s.parts) * PA_ROWS;
         for (int i = (blockIdx.x - head * p.alone) * PA_THREADS + threadIdx.x; i < kept * (HS / 4); i += p.alone * PA_THREADS) {
             const int r = i / (HS / 4), d = i % (HS / 4) * 4;
-            float m[PA_CLUSTER], l[PA_CLUSTER], top = -INFINITY, all = 0.0f, x[4] = {};
+            float m[PA_CLUSTER], l[PA_CLUSTER], top = LOWEST, all = 0.0f, x[4] = {};
             float4 v[PA_CLUSTER];
 #pragma unroll
             for (int k = 0; k < PA_CLUSTER; ++k) {
@@ -832,7 +909,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant_
 #pragma unroll
             for (int k = 0; k < PA_CLUSTER; ++k) {
                 if (l[k] < 0.0f) continue;
-                const float by = l[k] == 0.0f ? 0.0f : l[k] == l[k] ? exp2f(m[k] - top) : l[k];
+                const float by = exp2f(m[k] - top);
                 all = fmaf(l[k], by, all);
                 x[0] = fmaf(v[k].x, by, x[0]);
                 x[1] = fmaf(v[k].y, by, x[1]);

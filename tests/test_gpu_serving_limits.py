@@ -141,3 +141,47 @@ def test_a_value_that_is_not_finite_is_seen_however_small_its_weight(bmb, cuda, 
         loose = torch.zeros(2, heads, hs, dtype=torch.bool, device="cuda")
         loose[0, :group, 5] = loose[0, -group:, 9] = loose[1, -group:, 3] = True
         check_limits(bmb, torch, q, k, v, [longest, longest - 1], 1.0, width, loose)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("heads,kv,hs,longest,width", FORMS)
+@pytest.mark.parametrize("what", ["key", "value", "query", "both"])
+def test_infinities_do_what_they_do_in_the_formula(bmb, cuda, name, heads, kv, hs, longest, width, what):
+    """Keys, values and queries of both infinities, beside queries and weights of both signs and zeros: scores of -infinity have no weight, those of
+    infinity and NaN leave NaN, an infinite value stays what it is unless it meets the other infinity."""
+    torch, inf = cuda, float("inf")
+    for seed in range(3):
+        q, k, v = texts(torch, name, 3, longest, heads, kv, hs, seed)
+        a, b = longest // 5, longest - 3
+        if what == "key":
+            q[:, :, 3] = q[:, :, 3].abs()                     # (whole texts whose scores are -infinity, and others whose are infinity)
+            q[1, 0, 4] = 0.0
+            k[0, a, 0, 3], k[1, b, kv - 1, 4], k[2, a, 0, 5], k[2, b, 0, 6] = -inf, inf, inf, -inf
+            k[0, b, 0, 3] = -inf
+        elif what == "value":
+            v[0, a, 0, 3], v[0, b, 0, 4], v[1, a, kv - 1, 5], v[1, b, kv - 1, 5], v[2, b, 0, 0] = inf, -inf, inf, -inf, inf
+        elif what == "query":
+            q[0, 0, 3], q[1, heads - 1, 4], q[2, 0, 0] = inf, -inf, float("nan")
+        else:
+            q[:, :, 3] = 1.0
+            k[0, :, 0, 3] = -inf                              # nothing of a weight is left
+            k[1, a:, :, 3] = -inf
+            v[1, 0, 0, 7] = inf
+        check_limits(bmb, torch, q, k, v, [longest, longest, longest - 1], hs ** -0.5, width)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("heads,kv,hs,longest,width", FORMS)
+def test_the_largest_numbers_are_finite(bmb, cuda, name, heads, kv, hs, longest, width):
+    """The largest and lowest value of the cache's type among values, and keys and queries of that size whose scores are ordinary."""
+    torch = cuda
+    for seed in range(2):
+        q, k, v = texts(torch, name, 2, longest, heads, kv, hs, seed)
+        most = torch.finfo(k.dtype).max
+        v[0, longest // 2, 0, 3], v[0, 1, kv - 1, 4], v[1, longest - 2, 0, 5] = most, -most, most
+        check_limits(bmb, torch, q, k, v, [longest, longest - 1], hs ** -0.5, width)
+        k[0, longest // 3, :, 2], k[1, 0, :, 2] = most, -most
+        q[:, :, 2] = 8.0 / most
+        check_limits(bmb, torch, q, k, v, [longest, longest - 1], hs ** -0.5, width)
+        q[:, :, 2], k[:, :, :, 2] = torch.finfo(torch.float32).max, 0.0
+        check_limits(bmb, torch, q, k, v, [longest, longest - 1], hs ** -0.5, width)
