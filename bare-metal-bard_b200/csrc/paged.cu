@@ -296,22 +296,35 @@ struct Attend {
     Parts w;
 };
 
+// A block's static shared memory.
+struct AttendShared {
+    float weight[2 * PA_WARPS][PA_ROWS];                                         // (aligned; and at the start:)
+    struct RunBegin { long long in; int request; };                              // `in` places behind the first one of this request
+    int4 part_of[PA_WARPS][2];                                                   // request, virtual head, 1 begins + 2 ends there, 1 (0: none)
+    long long warp_total[PA_WARPS];                                              // (at the start)
+    float part_m[PA_WARPS][2][PA_ROWS], part_l[PA_WARPS][2][PA_ROWS];
+    int last_block[PA_WARPS + 1];                                                // that has a part of the head a warp has begun and not ended
+};
+static_assert(sizeof(AttendShared::weight) >= PA_WARPS * sizeof(AttendShared::RunBegin), "");
+// Two blocks an SM: of its 228 KB each takes 1 KB beside its own, of which the static part is padded to the dynamic one's boundary.
+static_assert(PA_BLOCKS * (PA_SMEM + 1024 + (sizeof(AttendShared) + 127) / 128 * 128) <= 228 * 1024, "");
+
 template <typename T, int HS>
-__global__ void __launch_bounds__(PA_THREADS, 2) attend_k(const __grid_constant__ Attend p) {
+__global__ void __launch_bounds__(PA_THREADS, PA_BLOCKS) attend_k(const __grid_constant__ Attend p) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     constexpr int KEYS = PA_TILE / (HS * (int)sizeof(T)), NT = KEYS / 8;         // keys a tile, and tiles of 8
     constexpr int UNITS = HS * (int)sizeof(T) / 16;                              // 16-byte units of a row
     constexpr float SHIFT = !F32 && !BF ? 14.0f : 0.0f;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ long long warp_total[PA_WARPS];                                   // (at the start)
-    __shared__ float part_m[PA_WARPS][2][PA_ROWS], part_l[PA_WARPS][2][PA_ROWS];
-    __shared__ int4 part_of[PA_WARPS][2];                                        // request, virtual head, 1 begins + 2 ends there, 1 (0: none)
-    __shared__ __align__(16) float weight[2 * PA_WARPS][PA_ROWS];                // (and at the start:)
-    struct RunBegin { long long in; int request; };                              // `in` places behind the first one of this request
-    RunBegin *run_begin = reinterpret_cast<RunBegin *>(weight);
-    static_assert(sizeof(weight) >= PA_WARPS * sizeof(RunBegin), "");
-    __shared__ int last_block[PA_WARPS + 1];                                      // that has a part of the head a warp has begun and not ended
+    __shared__ __align__(16) AttendShared sh;
+    auto &weight = sh.weight;
+    auto &part_of = sh.part_of;
+    auto &warp_total = sh.warp_total;
+    auto &part_m = sh.part_m;
+    auto &part_l = sh.part_l;
+    auto &last_block = sh.last_block;
+    auto *run_begin = reinterpret_cast<AttendShared::RunBegin *>(weight);
     int *group_of = reinterpret_cast<int *>(warp_total), &groups = last_block[PA_WARPS];      // first entry, last one << 8, what they say together << 16
     static_assert(sizeof(warp_total) >= 2 * PA_WARPS * sizeof(int), "");
 
@@ -1032,7 +1045,7 @@ Shape attend_shape(int n, int heads, int kv_heads, int hs, int type, int cap) {
 template <typename T, int HS>
 int run_attend(Attend &p, cudaStream_t st) {
     const int blocks = attend_blocks(), rows = p.s.group < PA_ROWS ? p.s.group : PA_ROWS;
-    // staged queries where two blocks still fit an SM (228 KB, of which a block takes 1 KB and the static 1.2 KB besides)
+    // staged queries where two blocks still fit an SM
     const size_t part = rows * HS * sizeof(float), least = (size_t)PA_WARPS * (PA_STAGES * 2 * PA_TILE + part);
     p.staged = least + PA_WARPS * 2 * part <= PA_SMEM;
     p.aligned_q = ((uintptr_t)p.q & 15) == 0 && p.q_stride % 4 == 0;
