@@ -331,7 +331,8 @@ int bmb_paged_kv_write(const bmb_kv_cache *cache, const float *k, const float *v
 /* Attention of one new token of each of n requests over the tokens that the cache holds of it (its own included, once written):
  * out[i][h] = sum_j softmax_j(scale q[i][h] . k_j) v_j over j < lens[i] (clamped to the table), where heads is a multiple of the
  * cache's and query head h reads cache head h / (heads / cache->heads).  Rows of q and out are q_stride and out_stride floats
- * apart (q may lie in rows of a qkv product; out must not overlap it).  lse ([n][heads], may be NULL) receives the natural
+ * apart, row i being request i's (q may lie in rows of a qkv product, if these are one for each request, as where each adds one token in a step;
+ * otherwise request i's newest token is in row starts[i + 1] - 1 of the new tokens', and q is gathered from there; out must not overlap q).  lse ([n][heads], may be NULL) receives the natural
  * logarithm of the sum of exponentials.  Row i of tables ([n][max_pages]) names request i's pages; tokens in pages that are
  * not of the pool count as absent, and are not read.  Where nothing is left, out is 0 and lse -infinity.
  * workspace: bmb_paged_attention_workspace bytes on the device, 16-byte aligned, of this call's own until it has run (two
