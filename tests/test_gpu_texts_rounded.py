@@ -33,8 +33,8 @@ class RoundedTexts64(Texts64):
 # layers) lie on two sides of a rounding border.  bf16: steps of 2^-8 at most, so one element in 2^11, 2 of a layer's 2 * 24 * 96; a value's
 # moves its column by 2^-8 / 20 of itself, a key's a score by 2^-8 / sqrt(hs), either 2e-4 at most behind a softmax over 20 tokens, so a cumulative
 # probability by some 5e-4 over three layers, of which four times are allowed.  fp16: steps of an eighth, 8 times as many of them, which add up like
-# sqrt(8): 3 / 8 of that, and the fp32 error itself besides.  How many draws: of up to 300 borders each moves by 1e-4 on average, 3 %, of
-# which three times are allowed.
+# sqrt(8): 3 / 8 of that, and the fp32 error itself besides.  How many draws: as over an fp32 cache.  (Measured: none of 475; of a model that rounds
+# keys and values to another type 5 to 16 of a configuration's, or one beyond the border.)
 @pytest.mark.parametrize("heads,hs,B,T,V,flash", CONFIGS)
 @pytest.mark.parametrize("penalties", [(1.0, 0.0, 0.0), (1.3, 0.4, 0.2)])
 @pytest.mark.parametrize("cache,near", [("TYPE_BF16", 2e-3), ("TYPE_FP16", 1e-3)])
@@ -54,5 +54,5 @@ def test_texts_over_a_cache_of_16_bits(bmb, cuda, heads, hs, B, T, V, flash, pen
     for i, (p, o) in enumerate(zip(prompts, out)):
         m.prompt = len(p)
         close += check_draws(m, p, o, 11 + i, 0.9, *penalties, near)
-    assert close <= 5 * steps // 11
+    assert close <= 3
     t.close()
