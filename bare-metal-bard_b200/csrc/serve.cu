@@ -3,6 +3,7 @@
 // for one text; a draw here is its draw.
 #include "common.cuh"
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <numeric>
 #include <random>
@@ -142,7 +143,7 @@ int generate_texts(const ServeModel &m, int n, const int *host_prompts, int prom
         BMB_CUDA(cudaMemcpyAsync(dst, src, size, cudaMemcpyHostToDevice, st));      // (nothing that it reads changes before the next synchronise)
         return BMB_OK;
     };
-    std::vector<int> tokens(rows, 0), history((size_t)n * longest, 0), ids(pages), ones(n, 1), none(n, 0), last(n), ended(n, 0);
+    std::vector<int> tokens(rows, 0), history((size_t)n * longest, 0), ids(pages), ones(n, 1), last(n), ended(n, 0);
     std::vector<float> same(3 * (size_t)n), probs((size_t)n * Vp);
     struct Idle {                        // arena and vectors go when nothing reads or writes them any more
         cudaStream_t st;
@@ -268,8 +269,11 @@ int generate_texts(const ServeModel &m, int n, const int *host_prompts, int prom
 
 int draw_token(float *probs, int V, float temperature, float coin) {
     if (temperature != 1.0f) {
+        // Cold draws: where even the largest power is below fp32's normal numbers (0.1^100), the powers are those of shares of the largest.
+        const float top = *std::max_element(probs, probs + V);
+        const float unit = top > 0.0f && powf(top, 1.0f / temperature) < FLT_MIN ? top : 1.0f;
         float sum = 0.0f;
-        for (int i = 0; i < V; ++i) { probs[i] = powf(probs[i], 1.0f / temperature); sum += probs[i]; }
+        for (int i = 0; i < V; ++i) { probs[i] = powf(probs[i] / unit, 1.0f / temperature); sum += probs[i]; }
         for (int i = 0; i < V; ++i) probs[i] /= sum;
     }
     float cdf = 0.0f;

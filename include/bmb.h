@@ -509,7 +509,9 @@ int bmb_trainer_load(bmb_trainer *t, const char *path, int load_optimizer_state,
 int bmb_trainer_next_token_probs(bmb_trainer *t, const int *host_tokens, int pos, float *host_probs);
 /* The reference's generate(): starts from start_token, draws `steps` tokens with mt19937(seed) and a
  * uniform float per token, probabilities raised to 1/temperature and renormalised when temperature != 1,
- * the window sliding once the context is full.  host_tokens_out receives the drawn token ids. Blocks. */
+ * the window sliding once the context is full.  host_tokens_out receives the drawn token ids. Blocks.
+ * Where the largest probability's power 1 / temperature is below fp32's normal numbers (where the reference divides by a sum of 0 and draws the last token), powers
+ * are those of shares of the largest, so that a cold draw is of the likeliest tokens. */
 int bmb_trainer_generate(bmb_trainer *t, int start_token, int steps, unsigned seed, float temperature,
                          int *host_tokens_out);
 /* Several texts at once: text i begins with the host_prompt_lens[i] (at least 1) tokens of row i of host_prompts ([n][prompt_stride]) and draws
