@@ -129,14 +129,14 @@ struct Run {
         }
         return (float)(total / n_batches);
     }
+    bool together() const { return o.texts > 1 || o.repetition != 1.0f || o.frequency != 0.0f || o.presence != 0.0f; }
     std::string sample(int len, unsigned seed) {
         int start = 0;
         for (size_t i = 0; i < corpus.itos.size(); ++i)
             if (corpus.itos[i] == '\n') { start = (int)i; break; }
-        const bool together = o.texts > 1 || o.repetition != 1.0f || o.frequency != 0.0f || o.presence != 0.0f;
-        if (together) len = std::min(len, o.T - 1);
+        if (together()) len = std::max(std::min(len, o.T - 1), 0);
         std::vector<int> toks((size_t)std::max(len, 1) * o.texts);
-        if (together) {
+        if (together()) {
             const std::vector<int> starts(o.texts, start), ones(o.texts, 1);
             const bmb_batch_sampling how{o.temperature, o.repetition, o.frequency, o.presence, -1, BMB_TYPE_FP32};
             CHECK(bmb_trainer_generate_batch(t, o.texts, starts.data(), 1, ones.data(), len, seed, &how, toks.data()));
@@ -262,6 +262,9 @@ int main(int argc, char **argv) {
     printf("memory    %.1f MB forward activations, %.1f MB backward scratch\n", act_mb, gact_mb);
     printf("total     %.2f GB resident (params+grads+adam+activations+scratch)\n", (4.0 * param_mb + act_mb + gact_mb) / 1024.0);
     if (o.alloc_only) { bmb_trainer_destroy(run.t); return 0; }
+
+    // What the drawing of several texts refuses (a head size, a penalty) is told now, not when the training has been done.
+    if (run.together() && o.sample_len > 0 && !o.synthetic) run.sample(1, o.seed);
 
     std::mt19937 rng(o.seed);
     std::vector<int> x((size_t)o.B * o.T), y((size_t)o.B * o.T);
