@@ -102,8 +102,8 @@ __global__ void __launch_bounds__(THREADS) assign_k(int *tables, int *lens_out, 
             lens_out[i] = served ? L + A : L;
             if (starts) starts[i] = begin_of[threadIdx.x];
         }
-        // (counted in 64 bits: the last step may end behind an int)
-        for (long long next = (long long)chunk_begin + me * THREADS + threadIdx.x; next < chunk_end; next += BLOCKS * THREADS) {
+        // (unsigned: the last step may end behind an int, by no more than a stretch)
+        for (unsigned next = (unsigned)chunk_begin + me * THREADS + threadIdx.x; next < (unsigned)chunk_end; next += BLOCKS * THREADS) {
             const int t = (int)next;
             int r = 0;                                        // the last request that begins at t or before it
 #pragma unroll
