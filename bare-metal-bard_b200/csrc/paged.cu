@@ -245,7 +245,7 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&out)[pieces])
     }
 }
 
-// n / d for 0 <= n < 2^31 and one d: the high half of n times ceil(2^(32 + bits) / d) - 2^32, bits such that 2^bits >= d.  (The division
+// n / d for 0 <= n < 2^31 and one d, by the method of Granlund and Montgomery (Division by invariant integers using multiplication, 1994): the high half of n times ceil(2^(32 + bits) / d) - 2^32, bits such that 2^bits >= d.  (The division
 // of unknown numbers takes 20 instructions.)
 struct Divide {
     unsigned by, mul, bits;

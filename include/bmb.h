@@ -324,7 +324,7 @@ int bmb_pages_release(int *free_pages, int *free_out, int *lens_out, const int *
                       const int *done, int n, int max_pages, int page_size, int pages, void *stream);
 /* Rows of keys and values (heads * head_size floats each, row_stride floats from one token to the next: 3C for rows of a qkv
  * product) into the slots of their tokens, rounded to the cache's type (to nearest even; beyond fp16's range: infinity).
- * Rows whose slot is negative or beyond the pool are left out.  Slots are distinct (of two rows with one slot either may be
+ * Rows whose slot is negative or beyond the pool are left out (but are there: all `tokens` rows may be read).  Slots are distinct (of two rows with one slot either may be
  * found there, or elements of both). */
 int bmb_paged_kv_write(const bmb_kv_cache *cache, const float *k, const float *v, long long row_stride, const int *slots,
                        int tokens, void *stream);
@@ -358,7 +358,7 @@ int bmb_paged_attention(float *out, float *lse, const float *q, const bmb_kv_cac
  *   repetition, frequency, presence   [n], need history
  *   bias_ids, bias   [n][bias_stride], the first bias_lens[i] count; of entries for one token the last; ids outside the vocabulary are passed over
  *   allowed   [n][allowed_stride] words: bit v % 32 of word v / 32 is 1 where token v may be drawn
- * Lengths are clamped to their strides. */
+ * Lengths are clamped to their strides.  Rows are there to their strides' ends: what is behind a length may be read, and means nothing. */
 typedef struct bmb_logit_rules {
     const int *history, *history_lens, *prompt_lens;
     const float *repetition, *frequency, *presence;
@@ -369,8 +369,8 @@ typedef struct bmb_logit_rules {
     int history_stride, bias_stride, allowed_stride;
 } bmb_logit_rules;
 /* out[i][v] for v < V, rows of both `stride` floats apart (out may be logits itself), in this order:
- *   x = logits;  v in the text: x > 0 ? x / repetition : x * repetition;  x -= frequency * (times v was drawn);
- *   v drawn at all: x -= presence;  x += bias;  not allowed: -infinity
+ *   x = logits;  v in the text: x > 0 ? x / repetition : x * repetition;  v drawn: x -= frequency * (times v was drawn), x -= presence;
+ *   v among the biases: x += bias;  not allowed: -infinity
  * every step rounded to fp32 by itself.  Columns from V on are left as they are in out.  A row whose mask allows nothing is -infinity
  * throughout. */
 int bmb_logits_adjust(float *out, const float *logits, int n, int V, long long stride, const bmb_logit_rules *rules, void *stream);
