@@ -337,7 +337,8 @@ int bmb_paged_kv_write(const bmb_kv_cache *cache, const float *k, const float *v
  * not of the pool count as absent, and are not read.  Where nothing is left, out is 0 and lse -infinity.
  * workspace: bmb_paged_attention_workspace bytes on the device, 16-byte aligned, of this call's own until it has run (two
  * streams, or two graphs that may run at once, have one each); its contents need no preparation and mean nothing afterwards.
- * Products and sums are of fp32 accuracy whatever the cache's type (with an fp16 cache elements of q are kept to 2^-39 of their row's largest).
+ * Products and sums are of fp32 accuracy whatever the cache's type (with an fp16 cache elements of q are kept to 2^-39 of their row's
+ * largest, with an fp32 cache elements of q, keys and values to 2^-136, where their second pieces end).
  * Infinities and NaN in q, and in keys and values that count, do what they do in fp32 in sum_j w_j v_j / sum_j w_j, w_j = exp(s_j - max s): a
  * score of NaN or +infinity makes a head's outputs and lse NaN, a score of -infinity has weight 0 (where no other token counts, nothing is left), an
  * infinite value makes its column infinite, or NaN beside the other infinity or with a weight that is 0.  Finite inputs have finite outputs as long as q . k, s / ln 2 and

@@ -83,9 +83,10 @@ def formula(torch, q, k, v, lens, scale):
     return out, bound, lse, lse_bound
 
 
-def check_limits(bmb, torch, q, k, v, lens, scale, width, loose=None):
+def check_limits(bmb, torch, q, k, v, lens, scale, width, loose=None, least=0.0):
     """Against the formula; `width`: pages of a row of the tables, by which attention is divided.  loose: (request, head, column) where NaN and
-    an infinity are alike, a weight being 0 in fp32 that is not in 64 bits."""
+    an infinity are alike, a weight being 0 in fp32 that is not in 64 bits.
+    least: what an output may be off besides."""
     n, heads, hs = q.shape
     longest, kv = k.shape[1:3]
     page = 16
@@ -104,7 +105,7 @@ def check_limits(bmb, torch, q, k, v, lens, scale, width, loose=None):
     bmb.call("bmb_paged_attention", out, lse, q, bmb.KvCache.of(*pools), tables.cuda(), i32(torch, lens), n, heads, heads * hs, heads * hs, width, scale, ws,
              ws.numel(), torch.cuda.current_stream().cuda_stream)
     want, bound, want_lse, lse_bound = formula(torch, q, k, v, lens, scale)
-    for got, want, bound in ((out.double(), want, bound), (lse.double(), want_lse, lse_bound)):
+    for got, want, bound in ((out.double(), want, bound + least), (lse.double(), want_lse, lse_bound)):
         finite = torch.isfinite(want)
         same = torch.where(finite, (got - want).abs() <= bound, (got == want) | (torch.isnan(got) & torch.isnan(want)))
         if loose is not None and got.dim() == 3:
@@ -185,3 +186,15 @@ def test_the_largest_numbers_are_finite(bmb, cuda, name, heads, kv, hs, longest,
         check_limits(bmb, torch, q, k, v, [longest, longest - 1], hs ** -0.5, width)
         q[:, :, 2], k[:, :, :, 2] = torch.finfo(torch.float32).max, 0.0
         check_limits(bmb, torch, q, k, v, [longest, longest - 1], hs ** -0.5, width)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("heads,kv,hs,longest,width", FORMS)
+def test_the_smallest_numbers(bmb, cuda, name, heads, kv, hs, longest, width):
+    """Values down to the type's smallest ones: of an fp32 value the second piece ends at 2^-136 (its 10 bits behind 2^-126), so each of the two
+    products that a weight's pieces make with it is off by that at most, and the weights' sum is 1."""
+    torch = cuda
+    q, k, v = texts(torch, name, 2, longest, heads, kv, hs)
+    tiny = torch.finfo(v.dtype).tiny
+    for scale in (64.0, 1.0, 2.0 ** -6):
+        check_limits(bmb, torch, q, k, (v.double() * tiny * scale).to(v.dtype), [longest, longest - 1], hs ** -0.5, width, least=2.0 ** -135)
