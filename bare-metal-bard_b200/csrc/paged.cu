@@ -87,7 +87,7 @@ int run_write(const bmb_kv_cache &c, const float *k, const float *v, long long r
 // has an infinity or a finite result.  A score of NaN, and an infinity or NaN in a sum of values, is still there when a head ends; what lost its sign would
 // be NaN too, so sums that are finite are right.  A warp that had others works on those heads (its parts of them) once more when its run is
 // done, a token at a time in plain fp32: what it leaves is what the formula gives.  The check at a head's end and the code for it cost
-// 0.1 us of the 6.2 of one text of 256 tokens, 0.15 of 15.3 where heads end with nearly every tile, and nothing that can be told of 99.
+// up to 0.1 us of the 6.2 of one text of 256 tokens, up to 0.3 of 15.3 where heads end with nearly every tile, and up to 0.5 % of 100.
 //
 // Bound by, and measured (us, caches cold): 609 MB of fp16, 8 requests of up to 32768 tokens, 32 heads on 8 of 128: 100, 6.1 TB/s, the loads.  203 MB of
 // fp32, 37 of up to 2777, 16 heads on 4 of 128: 44.5, and 101 MB of bf16, 64 of up to 1024, 12 heads of 64: 26.8: the loads alone take 40.8 and
@@ -97,7 +97,7 @@ constexpr int PA_WARPS = 4, PA_THREADS = 32 * PA_WARPS, PA_STAGES = 3, PA_TILE =
 constexpr int PA_BLOCKS = 2, PA_MOST_BLOCKS = 512;          // blocks an SM, and in all
 constexpr size_t PA_SMEM = 112 * 1024;                       // dynamic shared memory with which two blocks fit an SM
 constexpr int PA_CLUSTER = 8;
-constexpr float LOWEST = -3.402823466e38f;                   // number of fp32
+constexpr float LOWEST = -3.402823466e38f;                   // the lowest number of fp32
 
 // Blocks for each head, a cluster of them, or 0 for the line (below).  Where heads are few or short a cluster takes each alone: no line to find a
 // place in and no second launch, which together are 2 to 4 us of GPU time and 4 of the host's.  But then the longest head alone says how long it
@@ -245,8 +245,8 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&out)[pieces])
     }
 }
 
-// n / d for 0 <= n < 2^31 and one d, by the method of Granlund and Montgomery (Division by invariant integers using multiplication, 1994): the high half of n times ceil(2^(32 + bits) / d) - 2^32, bits such that 2^bits >= d.  (The division
-// of unknown numbers takes 20 instructions.)
+// n / d for 0 <= n < 2^31 and one d, by the method of Granlund and Montgomery (Division by invariant integers using multiplication, 1994): the
+// high half of n times ceil(2^(32 + bits) / d) - 2^32, bits such that 2^bits >= d.  (The division of unknown numbers takes 20 instructions.)
 struct Divide {
     unsigned by, mul, bits;
     Divide() = default;
